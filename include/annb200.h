@@ -567,6 +567,124 @@ typedef struct AnnB200TypedJob
 int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
 
 /*
+ * Softmax loss of queries over all of a shard's rows, for training the
+ * queries' encoder and the rows themselves (no counterpart in the reference,
+ * which searches rows that are trained elsewhere). The rows are the classes:
+ * with logits l_ij = scale * <query_i, row_j>,
+ *
+ *   lse_i  = log sum_j exp(l_ij)
+ *   loss_i = lse_i - l_i,target(i)
+ *
+ * The logits are never kept: like a search, the call walks the rows in
+ * pieces and keeps per query only a running maximum and sum, in FP32.
+ *
+ * dtype     ANNB200_F32, ANNB200_F16 or ANNB200_BF16: both operands and both
+ *           gradients. Products are summed in FP32 (FP32 operands as two
+ *           FP16 terms each, 22 bits). Finite FP32 values below 2^-17 of
+ *           their array's largest lose bits: each is held to within 2^-39 of
+ *           that largest.
+ * queries   device [nq] rows of dims values, query_stride values apart.
+ * rows      device [nrows] rows of dims values, row_stride values apart.
+ *           16-byte aligned FP16 / BF16 rows (address and stride) are read
+ *           where they are; others are copied into the workspace first.
+ * targets   device int64 [nq], row numbers. A negative target means none:
+ *           the loss is 0 and the query adds no gradient, whatever it holds.
+ *           A target >= nrows: status ANN_INVALID, loss NaN, no gradient.
+ * loss, lse device FP32 [nq]; either may be NULL. status: optional device
+ *           int32 [nq]. lse of a query without a target is computed too.
+ *
+ * AnnB200SoftmaxLossGrad: the gradient of sum_i grad_i * loss_i (grad:
+ * device FP32 [nq], NULL = all ones) from the same inputs and the lse that
+ * the forward call wrote:
+ *
+ *   G_ij = grad_i * (exp(l_ij - lse_i) - [j = target(i)])
+ *   dqueries_i = scale * sum_j G_ij row_j      [nq][dims]
+ *   drows_j    = scale * sum_i G_ij query_i    [nrows][dims]
+ *
+ * dense in dtype, overwritten; either may be NULL. The logits are computed
+ * again, piece by piece. Each piece of G is held in 16 bits for FP16 and BF16
+ * operands, two FP16 terms for FP32 operands. Results do not depend on timing: no
+ * atomics. A non-finite value makes non-finite what the formulas make so.
+ *
+ * Both calls only enqueue work on stream, on the current device, can be
+ * captured into a graph, and use workspace (device, 256-byte aligned, at
+ * least the bytes AnnB200SoftmaxLossWorkspace gives for the same job) until
+ * that work is done; calls that run at the same time need one each. nq <=
+ * 2^22, nrows < 2^31, dims <= 65,536. nq 0 does nothing; nrows 0 is
+ * ANN_INVALID. If a pipeline wait runs out inside a kernel (4 s), the
+ * outputs are NaN.
+ */
+#define ANNB200_BF16 5			/* operands of the calls below; not a shard's
+								 * row format */
+typedef struct AnnB200LossJob
+{
+	uint32_t	dtype;
+	uint32_t	dims;
+	uint32_t	nq;
+	float		scale;			/* finite */
+	uint64_t	nrows;
+	const void *queries;
+	uint64_t	query_stride;	/* in values, >= dims */
+	const void *rows;
+	uint64_t	row_stride;
+	const int64_t *targets;
+	float	   *loss;
+	float	   *lse;			/* written by the loss, read by the gradient */
+	int32_t    *status;
+	const float *grad;			/* the gradient call's from here on */
+	void	   *dqueries;
+	void	   *drows;
+	void	   *workspace;
+	uint64_t	workspace_bytes;
+} AnnB200LossJob;
+int			AnnB200SoftmaxLoss(const AnnB200LossJob *job, void *stream);
+int			AnnB200SoftmaxLossGrad(const AnnB200LossJob *job, void *stream);
+int			AnnB200SoftmaxLossWorkspace(const AnnB200LossJob *job, uint64_t *loss_bytes, uint64_t *grad_bytes);
+
+/*
+ * E4M3 with one FP32 scale per block of 128 values, where ANNB200_E4M3 has
+ * one per row: finer scales for rows and weights whose dimensions differ in
+ * size. Blocks are 1 x 128 (along a row, the last one shorter), or with
+ * square != 0 128 x 128 (rows and columns, the last ones smaller).
+ *
+ * AnnB200QuantizeBlocks: x is device [m] rows of k values (ANNB200_F32, F16
+ * or BF16), stride values apart. codes: device [m] rows of code_stride bytes
+ * (a multiple of 16, >= k); bytes k .. ceil(k/16)*16 - 1 are zeroed.
+ * scales: device [m][ceil(k/128)], or [ceil(m/128)][ceil(k/128)].
+ *   a     = max |x| over the block, at least 2^-100 unless it is 0
+ *   scale = a / 448 (1 for a block of zeros)
+ *   code  = the E4M3 number nearest to x * (448 / a), ties to even (where
+ *           the index builder's row quantizer, build_cuvs_index.py:296-348,
+ *           divides by the scale and sends ties down)
+ * A NaN makes its block's scale and codes NaN; an infinity makes the scale
+ * infinite and its own code NaN. Enqueued on stream, current device.
+ */
+int			AnnB200QuantizeBlocks(uint32_t dtype, const void *x, uint64_t stride, uint64_t m, uint32_t k,
+								  uint32_t square, uint8_t *codes, uint64_t code_stride, float *scales,
+								  void *stream);
+
+/*
+ * The product of two operands in that form (a score matrix of queries
+ * against rows, or a projection):
+ *
+ *   out[i][j] = sum over blocks b of a_scale(i, b) * b_scale(j, b)
+ *                 * sum over k in b of a[i][k] * b[j][k]
+ *
+ * a: m rows, b: n rows, of k codes, a_stride / b_stride bytes apart; codes
+ * 16-byte aligned, strides multiples of 16. Scales as AnnB200QuantizeBlocks
+ * writes them, 1 x 128 or (square != 0) 128 x 128, for each side alone. The
+ * sums within a block and over blocks are FP32; out (ANNB200_F32, F16 or
+ * BF16; rows out_stride values apart) is rounded once. Bytes past k are not
+ * read into the sums. m, n < 2^31, k <= 2^20; m or n 0 does nothing, k 0
+ * writes zeros. Enqueued on stream, current device; no workspace. A pipeline
+ * wait that runs out (4 s) leaves NaN.
+ */
+int			AnnB200MatmulBlocks(const uint8_t *a, uint64_t a_stride, const float *a_scales, uint32_t a_square,
+								const uint8_t *b, uint64_t b_stride, const float *b_scales, uint32_t b_square,
+								uint64_t m, uint64_t n, uint32_t k, uint32_t out_dtype, void *out,
+								uint64_t out_stride, void *stream);
+
+/*
  * Kernels this library has launched in this process (all devices). A caller
  * that times a region reads it before and after to count its launches.
  */

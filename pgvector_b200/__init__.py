@@ -14,6 +14,9 @@ Host-side mirror of the reference worker's interface for this path:
     (AnnIndexTreeMerge, ann/server/indexfile.c:3235-3258).
   * ``bitmap_rows`` - filter bitmap to row list (expand_*,
     ann/server/cuvs.c:1910-1968).
+  * ``softmax_loss`` / ``softmax_loss_grad`` - training queries and rows with
+    all rows as the classes; ``quantize_blocks`` / ``matmul_blocks`` - E4M3
+    with a scale per block of 128 and products in that form (ops.py).
 
 All compute runs in libannb200.so (AOT sm_100a CUDA); there is no CPU path.
 Tensors are torch CUDA tensors; torch only provides device memory and streams.
@@ -25,7 +28,7 @@ import numpy as np
 from . import _abi
 from ._lib import (OK, INVALID, UNSUPPORTED, NOMEM, BACKEND_ERROR, AnnB200Error, check, load)
 
-F32, F16, E4M3, NVFP4, BIT = 0, 1, 2, 3, 4
+F32, F16, E4M3, NVFP4, BIT, BF16 = 0, 1, 2, 3, 4, 5
 L2, IP, COSINE, HAMMING = 0, 1, 2, 3
 SHARD_HOST = 1
 WINDOW, FORCE_SIMT, FORCE_F16, BOUNDS_EXCHANGE = 1, 2, 8, 32
@@ -347,6 +350,9 @@ def search_typed(jobs):
     return out
 
 
-__all__ = ['Shard', 'search_typed', 'merge_topk', 'bitmap_rows', 'bitmap_rows_static', 'backend', 'search_gathered', 'device_count', 'load', 'check',
+from .ops import matmul_blocks, quantize_blocks, softmax_loss, softmax_loss_grad  # noqa: E402
+
+__all__ = ['softmax_loss', 'softmax_loss_grad', 'quantize_blocks', 'matmul_blocks', 'BF16',
+           'Shard', 'search_typed', 'merge_topk', 'bitmap_rows', 'bitmap_rows_static', 'backend', 'search_gathered', 'device_count', 'load', 'check',
            'AnnB200Error', 'F32', 'F16', 'E4M3', 'NVFP4', 'BIT', 'L2', 'IP', 'COSINE', 'HAMMING', 'WINDOW',
            'FORCE_SIMT', 'FORCE_F16', 'BOUNDS_EXCHANGE', 'OK', 'INVALID', 'UNSUPPORTED', 'NOMEM', 'BACKEND_ERROR']

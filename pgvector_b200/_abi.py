@@ -28,6 +28,16 @@ class AnnB200TypedJob(ctypes.Structure):
                 ('status', ctypes.c_int)]
 
 
+class AnnB200LossJob(ctypes.Structure):
+    """AnnB200LossJob of annb200.h: one softmax loss over a shard's rows."""
+    _fields_ = [('dtype', ctypes.c_uint32), ('dims', ctypes.c_uint32), ('nq', ctypes.c_uint32),
+                ('scale', ctypes.c_float), ('nrows', ctypes.c_uint64), ('queries', ctypes.c_void_p),
+                ('query_stride', ctypes.c_uint64), ('rows', ctypes.c_void_p), ('row_stride', ctypes.c_uint64),
+                ('targets', ctypes.c_void_p), ('loss', ctypes.c_void_p), ('lse', ctypes.c_void_p),
+                ('status', ctypes.c_void_p), ('grad', ctypes.c_void_p), ('dqueries', ctypes.c_void_p),
+                ('drows', ctypes.c_void_p), ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_uint64)]
+
+
 class AnnIndex(ctypes.Structure):
     _fields_ = [('generation', ctypes.c_uint64), ('rows', ctypes.c_uint32), ('dimensions', ctypes.c_uint32),
                 ('vectors', ctypes.POINTER(ctypes.c_float)), ('backend_state', ctypes.c_void_p)]

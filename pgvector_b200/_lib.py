@@ -66,6 +66,13 @@ SIGNATURES = {
                                    c_void_p, c_void_p, c_void_p]),
     'AnnB200StageTimes': (c_int, [c_void_p, c_void_p, c_uint32, c_int]),
     'AnnB200StageTiming': (c_int, [c_int]),
+    'AnnB200SoftmaxLoss': (c_int, [c_void_p, c_void_p]),
+    'AnnB200SoftmaxLossGrad': (c_int, [c_void_p, c_void_p]),
+    'AnnB200SoftmaxLossWorkspace': (c_int, [c_void_p, ctypes.POINTER(c_uint64), ctypes.POINTER(c_uint64)]),
+    'AnnB200QuantizeBlocks': (c_int, [c_uint32, c_void_p, c_uint64, c_uint64, c_uint32, c_uint32, c_void_p, c_uint64,
+                                      c_void_p, c_void_p]),
+    'AnnB200MatmulBlocks': (c_int, [c_void_p, c_uint64, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_uint32,
+                                    c_uint64, c_uint64, c_uint32, c_uint32, c_void_p, c_uint64, c_void_p]),
     'AnnB200CommId': (c_int, [c_void_p]),
     'AnnB200CommCreate': (c_int, [c_int, c_int, c_int, c_void_p, ctypes.POINTER(c_void_p)]),
     'AnnB200CommCreateAll': (c_int, [c_int, c_void_p, c_void_p]),
