@@ -582,7 +582,7 @@ int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
  *           gradients. Products are summed in FP32 (FP32 operands as two
  *           FP16 terms each, 22 bits). Finite FP32 values below 2^-17 of
  *           their array's largest lose bits: each is held to within 2^-39 of
- *           that largest.
+ *           that largest, and an infinite FP32 value counts as a NaN.
  * queries   device [nq] rows of dims values, query_stride values apart.
  * rows      device [nrows] rows of dims values, row_stride values apart.
  *           16-byte aligned FP16 / BF16 rows (address and stride) are read

@@ -2,6 +2,7 @@
 // types, conversions, argument checks' statuses.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -34,38 +35,19 @@ inline int op_launched(const char *what, unsigned long long kernels) {
   return OP_OK;
 }
 
-// C[m][n] = sum_k A(m, k) B(n, k) in FP32 on CUDA cores: 64 x 64 tiles, 256
-// threads of 4 x 4 sums. A, B: float (row, k); out(m, n, sum) for m < M, n < N.
-constexpr int kSimtTile = 64, kSimtK = 16;
-template <typename LA, typename LB, typename E>
-__global__ void __launch_bounds__(256) simt_gemm(LA a, LB b, int64_t M, int64_t N, int64_t K, E out) {
-  __shared__ float as[kSimtK][kSimtTile + 4], bs[kSimtK][kSimtTile + 4];
-  const int64_t m0 = (int64_t)blockIdx.y * kSimtTile, n0 = (int64_t)blockIdx.x * kSimtTile;
-  const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += kSimtK) {
-    for (int i = threadIdx.x; i < kSimtTile * kSimtK; i += 256) {
-      const int r = i / kSimtK, k = i % kSimtK;
-      as[k][r] = m0 + r < M && k0 + k < K ? a(m0 + r, k0 + k) : 0.0f;
-      bs[k][r] = n0 + r < N && k0 + k < K ? b(n0 + r, k0 + k) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSimtK; k++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = fmaf(as[k][tm * 4 + i], bs[k][tn * 4 + j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++)
-      if (m0 + tm * 4 + i < M && n0 + tn * 4 + j < N) out(m0 + tm * 4 + i, n0 + tn * 4 + j, acc[i][j]);
-}
-template <typename LA, typename LB, typename E>
-void launch_simt_gemm(LA a, LB b, int64_t M, int64_t N, int64_t K, E out, cudaStream_t st) {
-  const dim3 grid((unsigned)((N + kSimtTile - 1) / kSimtTile), (unsigned)((M + kSimtTile - 1) / kSimtTile));
-  simt_gemm<<<grid, 256, 0, st>>>(a, b, M, N, K, out);
+// A tensor map of an operand (shard.cu): boxes of 128 bytes x box_rows rows, 128-byte swizzle.
+bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
+                        uint64_t pitch, uint32_t box_rows);
+
+// SMs of the current device (a device's number never changes: asked once each).
+inline int op_sms() {
+  static int known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 0;
+  if (dev < 64 && known[dev]) return known[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev] = n;
+  return n;
 }
 
 }  // namespace annb200

@@ -1,0 +1,348 @@
+// pair_gemm.cuh - the tensor-core product loop of the operators: C = A B^T in
+// tiles of 256 rows by up to 256 columns, one tile at a time on a pair of SMs.
+//
+// A cluster of two CTAs works on one tile with tcgen05.mma.cta_group::2: each
+// CTA keeps its 128 rows of A and its half of B's columns in shared memory and
+// its 128 x N part of the FP32 sums in tensor memory. Against one CTA a tile
+// that halves what is loaded of B for the same products. Clusters are
+// persistent: cluster c takes items c, c + clusters, ... of the operator's
+// list. Roles in each CTA:
+//
+//   warps 0-7  epilogue: warp w reads tensor memory lanes 32 (w % 4) .. + 31
+//              and columns of the half w / 4, so a thread holds half a row.
+//   warp 8     TMA producer: the CTA's own tiles of each 128-byte K block, all
+//              completing on the leader CTA's barrier.
+//   warp 9     MMA issuer (leader CTA); tcgen05.commit frees the stage and
+//              publishes the sums in both CTAs.
+//
+// Two sums of 256 columns each let the epilogue of one run under the products
+// of the next. Operands are K-major (rows of K) or MN-major (K rows of M or N,
+// the transposed operand read as it lies), both in 128-byte-swizzled tiles.
+// With two planes an operand is the sum of two FP16 terms and a K step issues
+// three products of the four.
+//
+// Every wait is bounded; one that runs out ends the CTA's roles, and its
+// epilogue goes through its remaining items with NaN for their sums.
+#pragma once
+
+#include "ops.cuh"
+#include "tc.cuh"
+
+namespace annb200 {
+
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 32 * (kPairEpiWarps + 2);
+constexpr int kPairTileBytes = 128 * 128;     // 128 rows of 128 bytes (or 128 bytes wide, 128 K rows)
+constexpr int kPairSmem = 227 * 1024;
+
+struct PairItem {
+  int32_t a_row, b_row;   // first row of the tile's A and B (rows of the product, whichever way they lie)
+  int32_t k0;             // first K element
+  uint32_t kblocks;
+  uint32_t index;         // the operator's own
+};
+
+enum PairKind { PAIR_F16, PAIR_BF16, PAIR_E4M3 };
+
+// Instruction descriptor of a 256 x n tile over two SMs, FP32 sums.
+template <PairKind KIND, bool A_MN, bool B_MN>
+__device__ __forceinline__ uint32_t pair_idesc(uint32_t n) {
+  const uint32_t fmt = KIND == PAIR_BF16 ? 1u : 0u;   // F16 and E4M3 are both 0 in their kinds
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+         ((n >> 3) << 17) | ((256u >> 4) << 24);
+}
+
+// Descriptor of an MN-major operand in the 128-byte swizzle: 128-byte runs of
+// M/N, a row of them per K element; 8 K rows (1,024 bytes) apart along K,
+// `lead` bytes to the next 64 M/N elements.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lead) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <PairKind KIND>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (KIND == PAIR_E4M3)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrive on the barrier at this offset in both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void pair_commit(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_leader(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void remote_arrive(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// A tile into this CTA's dst; completes on the leader's barrier (a cluster address).
+__device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// Wait for a phase, at most kWaitNs and until another role of the CTA has given up.
+__device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+    for (int i = 0; i < 32; i++)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (globaltimer() - t0 > kWaitNs) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
+// What an epilogue warp needs of the loop: the sums of one accumulator after
+// another. `ok` stays false once a wait has run out.
+struct PairSums {
+  uint64_t *full;
+  uint32_t empty_leader;     // cluster address of the leader's empty[0]
+  volatile uint32_t *abort;
+  uint32_t tmem;
+  uint32_t n;
+  bool ok;
+  // Tensor memory address of the next accumulator's columns for this warp's lanes.
+  __device__ __forceinline__ uint32_t acquire() {
+    if (ok) ok = __all_sync(0xffffffffu, pair_wait(full + (n & 1), (n >> 1) & 1, abort));
+    tc_fence_after();
+    return tmem + (n & 1) * 256;
+  }
+  __device__ __forceinline__ void release() {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0 && ok) remote_arrive(empty_leader + (n & 1) * 8);
+    n++;
+  }
+  // 32 columns of this thread's row.
+  __device__ __forceinline__ void load(uint32_t addr, uint32_t (&r)[32]) {
+    if (ok) {
+      TMEM_LD32(addr, r);
+      tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j++) r[j] = 0x7fc00000u;
+    }
+  }
+};
+
+// The shared memory of an operator's loop: stages of (A planes, B planes), then barriers.
+template <class Op>
+struct PairShape {
+  static constexpr int A_BYTES = Op::PLANES * kPairTileBytes;
+  static constexpr int BAR_BYTES = 256;
+  // b_bytes: one plane's B tile of this CTA
+  static __host__ __device__ constexpr int stage(int b_bytes) { return A_BYTES + Op::PLANES * b_bytes; }
+  static __host__ __device__ constexpr int stages(int b_bytes) {
+    const int s = (kPairSmem - 1024 - BAR_BYTES - Op::SCRATCH) / stage(b_bytes);
+    return s < Op::MAX_STAGES ? s : Op::MAX_STAGES;
+  }
+  static constexpr int smem(int b_bytes) { return 1024 + stages(b_bytes) * stage(b_bytes) + BAR_BYTES + Op::SCRATCH; }
+};
+
+// Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), PER_BLOCK (an
+// accumulator per K block instead of per item), Args with maps a[PLANES],
+// b[PLANES] and bn (columns of a tile), items(args), item(args, i),
+// epilogue(args, item, sums, scratch, rank).
+template <class Op>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    pair_gemm(const __grid_constant__ typename Op::Args args) {
+  using Shape = PairShape<Op>;
+  constexpr int PLANES = Op::PLANES;
+  constexpr int KE = Op::KIND == PAIR_E4M3 ? 128 : 64;   // K elements of a block
+  constexpr int MAXS = Op::MAX_STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t b_bytes = args.bn * 64;                 // bn / 2 rows (or columns) of 128 bytes each K block
+  const uint32_t stage_bytes = Shape::stage(b_bytes);
+  const uint32_t stages = Shape::stages(b_bytes);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + stages * stage_bytes);
+  uint64_t *empty = full + MAXS;
+  uint64_t *tfull = empty + MAXS;
+  uint64_t *tempty = tfull + 2;
+  uint64_t *drain = tempty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile uint32_t *abort = tmem_slot + 1;
+  static_assert((2 * MAXS + 5) * 8 + 8 <= Shape::BAR_BYTES, "barriers");
+  uint8_t *scratch = reinterpret_cast<uint8_t *>(full) + Shape::BAR_BYTES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const uint32_t items = Op::items(args);
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < stages; s++) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(tfull + b, 1);
+      mbar_init(tempty + b, 2 * kPairEpiWarps);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (uint32_t i = cluster; i < items && ok; i += clusters) {
+        const PairItem w = Op::item(args, i);
+        const int32_t ar = w.a_row + (int32_t)rank * 128, br = w.b_row + (int32_t)(rank * (args.bn / 2));
+        for (uint32_t kb = 0; kb < w.kblocks; kb++, it++) {
+          const uint32_t s = it % stages;
+          if (!pair_wait(empty + s, ((it / stages) & 1) ^ 1, abort)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = map_to_leader(smem_u32(full + s));
+          if (rank == 0) mbar_expect_tx(full + s, 2 * stage_bytes);
+          const int32_t k = w.k0 + (int32_t)(kb * KE);
+          const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
+#pragma unroll
+          for (int p = 0; p < PLANES; p++) {
+            if (Op::A_MN) {
+              pair_load(a + p * kPairTileBytes, &args.a[p], ar, k, bar);
+              pair_load(a + p * kPairTileBytes + 8192, &args.a[p], ar + 64, k, bar);
+            } else {
+              pair_load(a + p * kPairTileBytes, &args.a[p], k, ar, bar);
+            }
+            if (Op::B_MN) {
+              for (uint32_t c = 0; c < args.bn / 2; c += 64)
+                pair_load(b + p * b_bytes + c * 128, &args.b[p], br + (int32_t)c, k, bar);
+            } else {
+              pair_load(b + p * b_bytes, &args.b[p], k, br, bar);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = pair_idesc<Op::KIND, Op::A_MN, Op::B_MN>(args.bn);
+      constexpr uint32_t A_STEP = Op::A_MN ? 2048 : 32, B_STEP = Op::B_MN ? 2048 : 32;
+      uint32_t it = 0, acc = 0;
+      bool ok = true;
+      for (uint32_t i = cluster; i < items && ok; i += clusters) {
+        const PairItem w = Op::item(args, i);
+        for (uint32_t kb = 0; kb < w.kblocks; kb++, it++) {
+          const bool first = Op::PER_BLOCK || kb == 0, last = Op::PER_BLOCK || kb + 1 == w.kblocks;
+          if (first && !pair_wait(tempty + (acc & 1), ((acc >> 1) & 1) ^ 1, abort)) {
+            ok = false;
+            break;
+          }
+          const uint32_t s = it % stages;
+          if (!pair_wait(full + s, (it / stages) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + (acc & 1) * 256;
+          const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
+          auto adesc = [&](uint32_t p, uint32_t kk) {
+            const uint32_t at = a + p * kPairTileBytes + kk * A_STEP;
+            return Op::A_MN ? sw128_mn_desc(at, 8192) : sw128_desc(at);
+          };
+          auto bdesc = [&](uint32_t p, uint32_t kk) {
+            const uint32_t at = b + p * b_bytes + kk * B_STEP;
+            return Op::B_MN ? sw128_mn_desc(at, 8192) : sw128_desc(at);
+          };
+#pragma unroll
+          for (uint32_t kk = 0; kk < 4; kk++) {
+            pair_mma<Op::KIND>(d, adesc(0, kk), bdesc(0, kk), idesc, !(first && kk == 0));
+            if (PLANES == 2) {   // high by low and low by high terms; low by low is below FP32's half step
+              pair_mma<Op::KIND>(d, adesc(0, kk), bdesc(1, kk), idesc, 1u);
+              pair_mma<Op::KIND>(d, adesc(1, kk), bdesc(0, kk), idesc, 1u);
+            }
+          }
+          pair_commit(empty + s);
+          if (last) {
+            pair_commit(tfull + (acc & 1));
+            acc++;
+          }
+        }
+      }
+      // the MMAs issued have ended, and the loads in flight have landed, before anything is freed
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain))
+                   : "memory");
+      uint64_t t0 = globaltimer();
+      while (!mbar_try_wait(drain, 0) && globaltimer() - t0 < kWaitNs) {
+      }
+      if (*abort) {
+        t0 = globaltimer();
+        for (uint32_t s = 0; s < stages; s++)
+          for (uint32_t parity = 0; parity < 2; parity++)
+            while (!mbar_try_wait(full + s, parity) && globaltimer() - t0 < kWaitNs) {
+            }
+      }
+    }
+    __syncwarp();
+  } else {
+    PairSums sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
+    for (uint32_t i = cluster; i < items; i += clusters) Op::epilogue(args, Op::item(args, i), sums, scratch, rank);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// One cluster per pair of SMs, or per item where there are fewer.
+template <class Op>
+cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, cudaStream_t st) {
+  const int b_bytes = (int)args.bn * 64;
+  const int smem = PairShape<Op>::smem(b_bytes);
+  cudaError_t e = cudaFuncSetAttribute(pair_gemm<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const uint32_t clusters = items < (uint32_t)(sms / 2) ? items : (uint32_t)(sms / 2);
+  pair_gemm<Op><<<2 * clusters, kPairThreads, smem, st>>>(args);
+  return cudaGetLastError();
+}
+
+}  // namespace annb200

@@ -45,6 +45,7 @@
 #include <cstdlib>
 
 #include "internal.cuh"
+#include "tc.cuh"
 
 namespace annb200 {
 
@@ -57,7 +58,6 @@ constexpr int B_BYTES = MAXBN * 128;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int EPI_BUF = 256;      // staged appends a warp buffers before a flush
 constexpr int TMEM_COLS = 512;
-constexpr unsigned long long kWaitNs = 4000000000ull;
 // E4M3 rows on FP8 tensor cores (see TcCfg<QF8>)
 constexpr int QF8 = 0x20 | DT_E4M3;
 
@@ -73,31 +73,6 @@ struct TcArgs {
   int32_t q_lo_row;    // FP8 scan: row of the query map holding the low terms' first query
   uint32_t pf_tiles;   // gathered FP16 rows: L2 prefetch this many of the CTA's tiles ahead
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ uint64_t globaltimer() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 
 // Wait for the phase of `parity` to complete; false once `limit_ns` passes
 // or another role has aborted.
@@ -117,27 +92,6 @@ __device__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abo
   }
 }
 
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-               : "memory");
-}
-
-// A (box rows) x 64 tile at (x, y) of a 2-D tensor into dst; completes on bar.
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y,
-                                            uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    smem_u32(bar))
@@ -173,18 +127,6 @@ __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint6
       : "memory");
 }
 
-// Shared-memory matrix descriptor of a K-major operand tile in the 128-byte
-// swizzle layout: rows of 128 bytes, 8-row (1024-byte) swizzle atoms stacked
-// along M/N (stride byte offset 1024), start address advanced 32 bytes per
-// 16-element K step inside the atom.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3fffu)   // start address
-         | ((uint64_t)1 << 16)                 // leading byte offset (unused for swizzled K-major)
-         | ((uint64_t)(1024 >> 4) << 32)       // stride byte offset
-         | ((uint64_t)1 << 46)                 // descriptor version (sm100)
-         | ((uint64_t)2 << 61);                // 128-byte swizzle
-}
-
 // Instruction descriptor: FP16 A and B, FP32 accumulator, both K-major.
 __device__ __forceinline__ uint32_t f16_idesc(uint32_t n) {
   return (1u << 4)                  // D format F32
@@ -206,19 +148,6 @@ __device__ __forceinline__ uint32_t i8_idesc(uint32_t n) {
          | ((n >> 3) << 17)         // N / 8
          | ((uint32_t)(BM >> 4) << 24);  // M / 16
 }
-
-#define TMEM_LD32(taddr, r)                                                                          \
-  asm volatile(                                                                                      \
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15," \
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                     \
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),        \
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),    \
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), \
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), \
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])                                         \
-      : "r"(taddr))
-
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Passing (query, v, position) triples staged in a warp's shared buffer
 // (warp-uniform slot arithmetic, no atomics) and flushed to the global

@@ -439,6 +439,13 @@ int report_error(int status, const char *fmt, ...) {
   return status;
 }
 void count_launches(unsigned long long n) { counted(n); }
+// A 2-D tensor [outer][inner] of 16-bit or (bytes 1) 8-bit values, pitch bytes
+// a row, read in 128-byte-swizzled boxes of 128 bytes x box_rows rows.
+bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
+                        uint64_t pitch, uint32_t box_rows) {
+  return bytes == 1 ? encode_u8_seg_map(map, base, inner, outer, pitch, box_rows)
+                    : encode_f16_map(map, base, inner, outer, pitch, box_rows);
+}
 }  // namespace annb200
 
 extern "C" const char *AnnB200LastError(void) { return g_error.c_str(); }

@@ -197,6 +197,12 @@ def test_non_finite_values_stay_with_what_holds_them(cuda, dtype):
     other = torch.arange(40, device='cuda') != 7
     assert bool(torch.isnan(loss[7])) and bool(torch.isnan(lse[7])) and bool(torch.isnan(dx[7]).all())
     assert torch.equal(loss[other], ok[0][other]) and torch.equal(dx[other], ok[2][other])
+    if dtype == 'f32':   # (held as two terms: an infinite value counts as a NaN)
+        w2 = w.clone()
+        w2[11, 5] = float('inf')
+        loss, lse = pb.softmax_loss(x, w2, t, scale=4.0)
+        assert bool(torch.isnan(lse).all())
+        return
     # a row of -inf has probability 0 for queries of positive values: the others' loss stays
     xp, wp = x.abs() + 0.01, w.clone()
     wp[11] = float('-inf')
