@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(256) pack_rows(const T *x, uint64_t stride, ui
 template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
 struct LogitsOp {
   static constexpr PairKind KIND = KIND_;
-  static constexpr bool A_MN = false, B_MN = false, PER_BLOCK = false;
-  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8, CHUNK = PLANES == 2 ? 1 : 4;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];
     uint32_t bn;
@@ -175,6 +175,7 @@ struct LogitsOp {
     const float *lse, *grad;
     O *g;                    // gradient: [query][ldg], PLANES planes
     uint64_t ldg, gplane;
+    float *gsum;             // [query][2 nt]: the stored G summed over a half tile
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
@@ -204,69 +205,85 @@ struct LogitsOp {
     }
     const int64_t col0 = (int64_t)w.b_row + half * 128;   // this thread's first row of W
     const int64_t at = tgt - col0;                        // the target's column, if in [0, 128)
-    const uint32_t tmem = sums.acquire();
+    float v[4][32];
+    sums.template total<CHUNK>(half * 128, w.kblocks, v);
     if (any) {
-      float m = -INFINITY, s = 0.0f;
+      float m = -INFINITY, s = 0.0f;   // of this thread's 128 columns
       const int64_t left = (int64_t)p.nrows - col0;       // columns that are rows of W
-#pragma unroll 1
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        if (left <= c0) break;
-        uint32_t r[32];
-        sums.load(tmem + half * 128 + c0, r);
-        const bool hit = at >= c0 && at < c0 + 32;
-        if (!GRAD) {
-          if (__any_sync(0xffffffffu, hit)) {
-            float t = 0.0f;
+      const bool hit = __any_sync(0xffffffffu, valid && at >= 0 && at < 128);
+      if (!GRAD) {
+        // in base 2; columns past the rows count for nothing
 #pragma unroll
-            for (int j = 0; j < 32; j++) t = at == c0 + j ? __uint_as_float(r[j]) * k : t;
-            if (hit && valid) p.tlogit[q] = t;
-          }
-          // `part`: the last columns are past the rows and count for nothing
-          auto take = [&](auto part) {
-            auto in = [&](int j) { return !decltype(part)::value || c0 + j < left; };
-            float top = -INFINITY;
+        for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (in(j)) top = fmaxf(top, __uint_as_float(r[j]) * k);
-            const float now = fmaxf(m, top);
-            const float base = now == -INFINITY ? 0.0f : now;
-            float e[4] = {s * exp2_approx(m - base), 0.0f, 0.0f, 0.0f};
+          for (int j = 0; j < 32; j++) v[c][j] *= k;
+        if (hit) {
+          float t = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (in(j)) e[j & 3] += exp2_approx(fmaf(__uint_as_float(r[j]), k, -base));
-            s = (e[0] + e[1]) + (e[2] + e[3]);
-            m = now;
-          };
-          if (left >= c0 + 32) take(std::false_type());
-          else take(std::true_type());
-        } else {
-          float v[32];
+          for (int c = 0; c < 4; c++)
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = exp2_approx(fmaf(__uint_as_float(r[j]), k, -lse2));
-          if (__any_sync(0xffffffffu, hit)) {
+            for (int j = 0; j < 32; j++) t = (int)at == c * 32 + j ? v[c][j] : t;
+          if (valid && at >= 0 && at < 128) p.tlogit[q] = t;
+        }
+        if (left < 128) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] -= at == c0 + j ? 1.0f : 0.0f;
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[c][j] = c * 32 + j < (int)left ? v[c][j] : -INFINITY;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) top[j & 3] = fmaxf(top[j & 3], v[c][j]);
+        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float base = m == -INFINITY ? 0.0f : m;
+        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) e[j & 3] += exp2_approx(v[c][j] - base);
+        s = (e[0] + e[1]) + (e[2] + e[3]);
+      } else {
+        O *row = p.g + (uint64_t)q * p.ldg + (col0 - (int64_t)p.first);
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[c][j] = exp2_approx(fmaf(v[c][j], k, -lse2));
+        if (hit) {
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[c][j] -= at == c * 32 + j ? 1.0f : 0.0f;
+        }
+        if (left < 128) {   // (the buffer goes to whole tiles; what is past the rows is not read)
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[c][j] = c * 32 + j < (int)left ? v[c][j] : 0.0f;
+        }
+#pragma unroll
+        for (int j0 = 0; j0 < 128; j0 += 8) {
+          alignas(16) O hi[8], lo[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const float f = kept ? v[j0 / 32][j0 % 32 + j] * g : 0.0f;
+            hi[j] = from_float<O>(f);
+            s += to_float(hi[j]);      // the sum of what is stored
+            if (PLANES == 2) {
+              lo[j] = from_float<O>(f - to_float(hi[j]));
+              s += to_float(lo[j]);
+            }
           }
           if (valid) {
-            O *row = p.g + (uint64_t)q * p.ldg + (col0 - (int64_t)p.first) + c0;
-#pragma unroll
-            for (int j0 = 0; j0 < 32; j0 += 8) {
-              alignas(16) O hi[8], lo[8];
-#pragma unroll
-              for (int j = 0; j < 8; j++) {
-                const float f = kept ? v[j0 + j] * g : 0.0f;
-                hi[j] = from_float<O>(f);
-                if (PLANES == 2) lo[j] = from_float<O>(f - to_float(hi[j]));
-              }
-              *reinterpret_cast<uint4 *>(row + j0) = *reinterpret_cast<uint4 *>(hi);
-              if (PLANES == 2) *reinterpret_cast<uint4 *>(row + p.gplane + j0) = *reinterpret_cast<uint4 *>(lo);
-            }
+            *reinterpret_cast<uint4 *>(row + j0) = *reinterpret_cast<uint4 *>(hi);
+            if (PLANES == 2) *reinterpret_cast<uint4 *>(row + p.gplane + j0) = *reinterpret_cast<uint4 *>(lo);
           }
         }
       }
+      if (GRAD && valid) p.gsum[(uint64_t)q * (2 * p.nt) + 2 * w.index + half] = s;
       if (!GRAD && valid) p.part[(uint64_t)(q - p.q0) * (2 * p.nt) + 2 * w.index + half] = make_float2(m, s);
     }
-    sums.release();
   }
 };
 
@@ -310,8 +327,8 @@ __global__ void __launch_bounds__(128) join_parts(const float2 *part, uint32_t n
 template <PairKind KIND_, int PLANES_>
 struct QueriesOp {
   static constexpr PairKind KIND = KIND_;
-  static constexpr bool A_MN = false, B_MN = true, PER_BLOCK = false;
-  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8;
+  static constexpr bool A_MN = false, B_MN = true;
+  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8, CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); W's rows from the piece's first on
     uint32_t bn;
@@ -333,16 +350,24 @@ struct QueriesOp {
     if (w.kblocks == 0) return;   // (a short last piece; its partial stays)
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t q = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
-    const uint32_t tmem = sums.acquire();
     const uint32_t cols = p.bn / 2;
+    float v[4][32];
+    uint32_t tmem = 0;
+    if (CHUNK) sums.template total<CHUNK + !CHUNK>(half * cols, w.kblocks, v);
+    else tmem = sums.acquire() + half * cols;
     float *row = p.part + ((uint64_t)w.index * p.nq + q) * p.dims;
     const bool vec = p.dims % 4 == 0;
-#pragma unroll 1
-    for (uint32_t c0 = 0; c0 < cols; c0 += 32) {
-      const uint32_t d0 = (uint32_t)w.b_row + half * cols + c0;
-      if (d0 >= p.dims) break;
+#pragma unroll
+    for (uint32_t c = 0; c < 4; c++) {
+      const uint32_t c0 = c * 32, d0 = (uint32_t)w.b_row + half * cols + c0;
+      if (c0 >= cols || d0 >= p.dims) break;
       uint32_t r[32];
-      sums.load(tmem + half * cols + c0, r);
+      if (CHUNK) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) r[j] = __float_as_uint(v[c][j]);
+      } else {
+        sums.load(tmem + c0, r);
+      }
       if (q >= p.nq) continue;
       if (vec) {
 #pragma unroll
@@ -363,7 +388,7 @@ struct QueriesOp {
           if (d0 + j < p.dims) row[d0 + j] = __uint_as_float(r[j]) + (p.add ? row[d0 + j] : 0.0f);
       }
     }
-    sums.release();
+    if (!CHUNK) sums.release();
   }
 };
 
@@ -371,8 +396,8 @@ struct QueriesOp {
 template <PairKind KIND_, int PLANES_, typename T>
 struct RowsOp {
   static constexpr PairKind KIND = KIND_;
-  static constexpr bool A_MN = true, B_MN = true, PER_BLOCK = false;
-  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8;
+  static constexpr bool A_MN = true, B_MN = true;
+  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8, CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); X
     uint32_t bn;
@@ -393,16 +418,24 @@ struct RowsOp {
     double f = p.scale * (double)grad_unit(p.maxima[MAX_GRAD]) / kGradScale;
     if (PLANES == 2) f *= (double)undo_scale(p.maxima[MAX_QUERIES]);
     const float factor = (float)f;
-    const uint32_t tmem = sums.acquire();
     const uint32_t cols = p.bn / 2;
+    float s[4][32];
+    uint32_t tmem = 0;
+    if (CHUNK) sums.template total<CHUNK + !CHUNK>(half * cols, w.kblocks, s);
+    else tmem = sums.acquire() + half * cols;
     T *row = p.out + (uint64_t)i * p.dims;
     const bool vec = p.dims % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-#pragma unroll 1
-    for (uint32_t c0 = 0; c0 < cols; c0 += 32) {
-      const uint32_t d0 = (uint32_t)w.b_row + half * cols + c0;
-      if (d0 >= p.dims) break;
+#pragma unroll
+    for (uint32_t c = 0; c < 4; c++) {
+      const uint32_t c0 = c * 32, d0 = (uint32_t)w.b_row + half * cols + c0;
+      if (c0 >= cols || d0 >= p.dims) break;
       uint32_t r[32];
-      sums.load(tmem + half * cols + c0, r);
+      if (CHUNK) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) r[j] = __float_as_uint(s[c][j]);
+      } else {
+        sums.load(tmem + c0, r);
+      }
       if (i >= p.rows) continue;
       constexpr int V = 16 / sizeof(T);
 #pragma unroll
@@ -419,23 +452,45 @@ struct RowsOp {
         }
       }
     }
-    sums.release();
+    if (!CHUNK) sums.release();
   }
 };
 
-// dX = scale * the partial sums, in order; zero for a query without a target.
+// A piece's sums of G into each query's (a warp a query).
+__global__ void __launch_bounds__(256) fold_sums(const float *gsum, uint32_t n, uint32_t nq, int add, double *total) {
+  const uint32_t q = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x % 32;
+  if (q >= nq) return;
+  double s = 0.0;
+  for (uint32_t i = lane; i < n; i += 32) s += gsum[(uint64_t)q * n + i];
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (lane == 0) total[q] = s + (add ? total[q] : 0.0);
+}
+
+// dX_i = scale * (the partial sums, in order, - (sum_j G_ij) w_target); zero for
+// a query without a target. G's exact rows sum to 0, the rounded ones do not,
+// and rows near each other (a cluster's) make sum_j G_ij w_j the small
+// difference of large terms: what is left of the sum would weigh in with a
+// whole row (10 times G's rounding where a cluster's rows differ by a tenth of
+// their length). With it taken off at the target, the sum is over
+// G_ij (w_j - w_target), and errors are relative to the differences.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t splits, uint32_t nq, uint32_t dims,
-                                                    double scale, const uint32_t *maxima, const int64_t *targets,
+                                                    double scale, const uint32_t *maxima, const double *total,
+                                                    const T *rows, uint64_t stride, const int64_t *targets,
                                                     uint64_t nrows, T *out) {
   const uint64_t n = (uint64_t)nq * dims;
-  double f = scale * (double)grad_unit(maxima[MAX_GRAD]) / kGradScale;
-  if (PLANES == 2) f *= (double)undo_scale(maxima[MAX_ROWS]);
+  const double f = scale * (double)grad_unit(maxima[MAX_GRAD]) / kGradScale;
   const float factor = (float)f;
+  const float undo = PLANES == 2 ? undo_scale(maxima[MAX_ROWS]) : 1.0f;
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-    float s = 0.0f;
-    for (uint32_t k = 0; k < splits; k++) s += part[k * n + i];
-    out[i] = from_float<T>(has_target(targets[i / dims], nrows) ? s * factor : 0.0f);
+    const uint32_t q = (uint32_t)(i / dims);
+    const int64_t t = targets[q];
+    float v = 0.0f;
+    if (has_target(t, nrows)) {
+      for (uint32_t k = 0; k < splits; k++) v += part[k * n + i];
+      v = fmaf(-(float)total[q], to_float(rows[(uint64_t)t * stride + (i - (uint64_t)q * dims)]), v * undo) * factor;
+    }
+    out[i] = from_float<T>(v);
   }
 }
 
@@ -461,7 +516,7 @@ struct Plan {
   int planes;
   uint32_t ld;             // values a packed row
   bool pack_x, pack_w;
-  uint64_t x, w, xscale, maxima, part, tlogit, g, dq, total;
+  uint64_t x, w, xscale, maxima, part, tlogit, g, gsum, gtotal, dq, total;
   uint32_t nt, chunk;      // forward: row tiles; queries a launch
   uint64_t piece;          // gradient: rows a piece
   uint32_t bn, dt, splits; // dimensions a tile, tiles, shares of a piece in dX
@@ -490,6 +545,8 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
     p.piece = std::max<uint64_t>(8192, kPieceBytes / (2 * p.planes * nq) / 256 * 256);
     p.piece = std::min<uint64_t>({p.piece, up(j.nrows, 256), 1u << 20});
     p.g = c.take(nq * p.piece * 2 * p.planes);
+    p.gsum = c.take(nq * (p.piece / 128) * 4);
+    p.gtotal = c.take(nq * 8);
     // 128 dimensions a tile where 256 would leave over an eighth of them empty
     const uint64_t full = up(j.dims, 256), fine = up(j.dims, 128);
     p.bn = fine * 8 < full * 7 ? 128 : 256;
@@ -633,6 +690,8 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   l.g = g;
   l.ldg = p.piece;
   l.gplane = gplane;
+  l.gsum = reinterpret_cast<float *>(ws + p.gsum);
+  double *gtotal = reinterpret_cast<double *>(ws + p.gtotal);
   for (uint64_t first = 0; first < j.nrows && e == cudaSuccess; first += p.piece) {
     const uint64_t n = std::min(p.piece, j.nrows - first);
     l.first = first;
@@ -652,8 +711,9 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       a.dims = j.dims;
       a.add = first != 0;
       a.part = dq;
+      fold_sums<<<(j.nq + 7) / 8, 256, 0, st>>>(l.gsum, 2 * l.nt, j.nq, a.add, gtotal);
       e = maps ? launch_pair<QOp>(a, a.mt * a.nt * a.splits, sms, st) : cudaErrorInvalidValue;
-      launches++;
+      launches += 2;
     }
     if (j.drows && e == cudaSuccess) {
       typename ROp::Args a = {};
@@ -676,7 +736,8 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   if (j.dqueries) {
     const uint64_t n = (uint64_t)j.nq * j.dims;
     join_queries<T, PLANES><<<(unsigned)std::min<uint64_t>((n + 255) / 256, 4736), 256, 0, st>>>(
-        dq, p.splits, j.nq, j.dims, (double)j.scale, maxima, j.targets, j.nrows, static_cast<T *>(j.dqueries));
+        dq, p.splits, j.nq, j.dims, (double)j.scale, maxima, gtotal, w, j.row_stride, j.targets, j.nrows,
+        static_cast<T *>(j.dqueries));
     launches++;
   }
   return op_launched("softmax loss gradient", launches);

@@ -16,7 +16,11 @@
 //              publishes the sums in both CTAs.
 //
 // Two sums of 256 columns each let the epilogue of one run under the products
-// of the next. Operands are K-major (rows of K) or MN-major (K rows of M or N,
+// of the next. The tensor cores cut off, and do not round, what falls below a
+// sum's last bit: over 48 steps of 16 (768 dimensions) that came to 1.4e-6 of
+// the sum, all of one sign, against 3e-8 in FP32 arithmetic. So an operator
+// whose result keeps 24 bits takes a sum over CHUNK K blocks and adds the
+// chunks up in registers, rounded. Operands are K-major (rows of K) or MN-major (K rows of M or N,
 // the transposed operand read as it lies), both in 128-byte-swizzled tiles.
 // With two planes an operand is the sum of two FP16 terms and a K step issues
 // three products of the four.
@@ -143,6 +147,34 @@ struct PairSums {
     if ((threadIdx.x & 31) == 0 && ok) remote_arrive(empty_leader + (n & 1) * 8);
     n++;
   }
+  // N x 32 columns from `at` on, of the item's whole K: its chunks, added up.
+  template <int CHUNK, int N>
+  __device__ __forceinline__ void total(uint32_t at, uint32_t kblocks, float (&v)[N][32]) {
+#pragma unroll
+    for (int c = 0; c < N; c++)
+#pragma unroll
+      for (int j = 0; j < 32; j++) v[c][j] = 0.0f;
+#pragma unroll 1
+    for (uint32_t kb = 0; kb < kblocks; kb += CHUNK) {
+      const uint32_t addr = acquire() + at;
+      if (ok) {
+#pragma unroll
+        for (int c = 0; c < N; c++) {
+          uint32_t r[32];
+          TMEM_LD32(addr + c * 32, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[c][j] += __uint_as_float(r[j]);
+        }
+      }
+      release();
+    }
+    const float poison = ok ? 0.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int c = 0; c < N; c++)
+#pragma unroll
+      for (int j = 0; j < 32; j++) v[c][j] += poison;
+  }
   // 32 columns of this thread's row.
   __device__ __forceinline__ void load(uint32_t addr, uint32_t (&r)[32]) {
     if (ok) {
@@ -169,8 +201,8 @@ struct PairShape {
   static constexpr int smem(int b_bytes) { return 1024 + stages(b_bytes) * stage(b_bytes) + BAR_BYTES + Op::SCRATCH; }
 };
 
-// Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), PER_BLOCK (an
-// accumulator per K block instead of per item), Args with maps a[PLANES],
+// Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
+// sum; 0: the item's), Args with maps a[PLANES],
 // b[PLANES] and bn (columns of a tile), items(args), item(args, i),
 // epilogue(args, item, sums, scratch, rank).
 template <class Op>
@@ -269,7 +301,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (uint32_t i = cluster; i < items && ok; i += clusters) {
         const PairItem w = Op::item(args, i);
         for (uint32_t kb = 0; kb < w.kblocks; kb++, it++) {
-          const bool first = Op::PER_BLOCK || kb == 0, last = Op::PER_BLOCK || kb + 1 == w.kblocks;
+          const bool first = Op::CHUNK ? kb % (Op::CHUNK + !Op::CHUNK) == 0 : kb == 0;
+          const bool last = kb + 1 == w.kblocks || (Op::CHUNK && (kb + 1) % (Op::CHUNK + !Op::CHUNK) == 0);
           if (first && !pair_wait(tempty + (acc & 1), ((acc >> 1) & 1) ^ 1, abort)) {
             ok = false;
             break;
