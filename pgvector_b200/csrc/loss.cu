@@ -28,7 +28,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial maxima and sums, at most about
-constexpr uint64_t kPieceBytes = 128ull << 20;  // G of a piece, where a piece has 8,192 rows by then
+constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece, where a piece has 8,192 rows by then
 constexpr uint32_t kPlanClusters = 74;          // clusters the plan splits for (148 SMs)
 
 enum { MAX_ROWS = 0, MAX_QUERIES = 1, MAX_GRAD = 2 };   // the workspace's maxima (float bits)
@@ -159,7 +159,8 @@ template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
 struct LogitsOp {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8, CHUNK = PLANES == 2 ? 1 : 4;
+  static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? kPairEpiWarps * kBoxBytes : 0, MAX_STAGES = 8;
+  static constexpr int CHUNK = PLANES == 2 ? 1 : 4;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];
     uint32_t bn;
@@ -173,8 +174,7 @@ struct LogitsOp {
     float2 *part;            // forward: [query - q0][2 nt]
     float *tlogit;           // [query]
     const float *lse, *grad;
-    O *g;                    // gradient: [query][ldg], PLANES planes
-    uint64_t ldg, gplane;
+    CUtensorMap g[PLANES];   // gradient: G of the piece
     float *gsum;             // [query][2 nt]: the stored G summed over a half tile
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
@@ -182,8 +182,8 @@ struct LogitsOp {
     const uint32_t n = i / p.mt, m = i % p.mt;   // a row tile against all queries before the next
     return {(int32_t)(p.q0 + m * 256), (int32_t)(p.first + (uint64_t)n * 256), 0, p.kblocks, n};
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums, uint8_t *,
-                                                  uint32_t rank) {
+  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums,
+                                                  uint8_t *scratch, uint32_t rank) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t q = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
     const bool valid = q < p.nq;
@@ -245,7 +245,7 @@ struct LogitsOp {
           for (int j = 0; j < 32; j++) e[j & 3] += exp2_approx(v[c][j] - base);
         s = (e[0] + e[1]) + (e[2] + e[3]);
       } else {
-        O *row = p.g + (uint64_t)q * p.ldg + (col0 - (int64_t)p.first);
+        // G; columns past the rows go to the buffer's end, which is not read
 #pragma unroll
         for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -256,30 +256,43 @@ struct LogitsOp {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[c][j] -= at == c * 32 + j ? 1.0f : 0.0f;
         }
-        if (left < 128) {   // (the buffer goes to whole tiles; what is past the rows is not read)
+        if (left < 128) {
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int j = 0; j < 32; j++) v[c][j] = c * 32 + j < (int)left ? v[c][j] : 0.0f;
         }
+        const BoxStore box{scratch + warp * kBoxBytes};
+        const int32_t x = (int32_t)(col0 - (int64_t)p.first), y = (int32_t)(q - lane);
+        // of a plane: the values it keeps, taken off v, and their sum
+        auto plane = [&](const CUtensorMap *map, bool last) {
+          float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int j0 = 0; j0 < 128; j0 += 8) {
-          alignas(16) O hi[8], lo[8];
+          for (int h = 0; h < 2; h++) {
+            BoxStore(box).reuse();
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float f = kept ? v[j0 / 32][j0 % 32 + j] * g : 0.0f;
-            hi[j] = from_float<O>(f);
-            s += to_float(hi[j]);      // the sum of what is stored
-            if (PLANES == 2) {
-              lo[j] = from_float<O>(f - to_float(hi[j]));
-              s += to_float(lo[j]);
+            for (int c = 0; c < 8; c++) {
+              alignas(16) O o[8];
+#pragma unroll
+              for (int j = 0; j < 8; j++) {
+                float &f = v[2 * h + c / 4][(c & 3) * 8 + j];
+                o[j] = from_float<O>(f);
+                const float kept_value = to_float(o[j]);
+                sum[j & 1] += kept_value;
+                if (!last) f -= kept_value;
+              }
+              BoxStore(box).put(c, *reinterpret_cast<uint4 *>(o));
             }
+            BoxStore(box).store(map, x + h * 64, y);
           }
-          if (valid) {
-            *reinterpret_cast<uint4 *>(row + j0) = *reinterpret_cast<uint4 *>(hi);
-            if (PLANES == 2) *reinterpret_cast<uint4 *>(row + p.gplane + j0) = *reinterpret_cast<uint4 *>(lo);
-          }
-        }
+          s += sum[0] + sum[1];
+        };
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[c][j] = kept ? v[c][j] * g : 0.0f;
+        plane(&p.g[0], PLANES == 1);
+        if (PLANES == 2) plane(&p.g[PLANES - 1], true);
       }
       if (GRAD && valid) p.gsum[(uint64_t)q * (2 * p.nt) + 2 * w.index + half] = s;
       if (!GRAD && valid) p.part[(uint64_t)(q - p.q0) * (2 * p.nt) + 2 * w.index + half] = make_float2(m, s);
@@ -328,7 +341,8 @@ template <PairKind KIND_, int PLANES_>
 struct QueriesOp {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = true;
-  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8, CHUNK = PLANES == 2 ? 2 : 0;
+  static constexpr int PLANES = PLANES_, SCRATCH = kPairEpiWarps * kBoxBytes, MAX_STAGES = 8;
+  static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); W's rows from the piece's first on
     uint32_t bn;
@@ -336,7 +350,7 @@ struct QueriesOp {
     uint32_t kblocks;        // of the piece
     uint32_t nq, dims;
     int add;                 // to what earlier pieces left
-    float *part;             // [splits][nq][dims]
+    CUtensorMap part;        // [splits][nq][dims]
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt * p.splits; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
@@ -345,8 +359,8 @@ struct QueriesOp {
     const uint32_t k1 = (uint32_t)((uint64_t)p.kblocks * (s + 1) / p.splits);
     return {(int32_t)((t / p.nt) * 256), (int32_t)((t % p.nt) * p.bn), (int32_t)(k0 * 64), k1 - k0, s};
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums, uint8_t *,
-                                                  uint32_t rank) {
+  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums,
+                                                  uint8_t *scratch, uint32_t rank) {
     if (w.kblocks == 0) return;   // (a short last piece; its partial stays)
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t q = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
@@ -355,38 +369,22 @@ struct QueriesOp {
     uint32_t tmem = 0;
     if (CHUNK) sums.template total<CHUNK + !CHUNK>(half * cols, w.kblocks, v);
     else tmem = sums.acquire() + half * cols;
-    float *row = p.part + ((uint64_t)w.index * p.nq + q) * p.dims;
-    const bool vec = p.dims % 4 == 0;
+    BoxStore box{scratch + warp * kBoxBytes};
 #pragma unroll
     for (uint32_t c = 0; c < 4; c++) {
-      const uint32_t c0 = c * 32, d0 = (uint32_t)w.b_row + half * cols + c0;
-      if (c0 >= cols || d0 >= p.dims) break;
+      const uint32_t d0 = (uint32_t)w.b_row + half * cols + c * 32;
+      if (c * 32 >= cols || d0 >= p.dims || q - lane >= p.nq) break;
       uint32_t r[32];
       if (CHUNK) {
 #pragma unroll
         for (int j = 0; j < 32; j++) r[j] = __float_as_uint(v[c][j]);
       } else {
-        sums.load(tmem + c0, r);
+        sums.load(tmem + c * 32, r);
       }
-      if (q >= p.nq) continue;
-      if (vec) {
+      box.reuse();
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          if (d0 + j < p.dims) {
-            float4 *o = reinterpret_cast<float4 *>(row + d0 + j);
-            float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
-                                   __uint_as_float(r[j + 3]));
-            if (p.add) {
-              const float4 u = *o;
-              v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
-            }
-            *o = v;
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; j++)
-          if (d0 + j < p.dims) row[d0 + j] = __uint_as_float(r[j]) + (p.add ? row[d0 + j] : 0.0f);
-      }
+      for (int j = 0; j < 8; j++) box.put(j, make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]));
+      box.store_sums(&p.part, (int32_t)d0, (int32_t)(q - lane), (int32_t)w.index, p.add != 0);
     }
     if (!CHUNK) sums.release();
   }
@@ -397,7 +395,8 @@ template <PairKind KIND_, int PLANES_, typename T>
 struct RowsOp {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = true, B_MN = true;
-  static constexpr int PLANES = PLANES_, SCRATCH = 0, MAX_STAGES = 8, CHUNK = PLANES == 2 ? 2 : 0;
+  static constexpr int PLANES = PLANES_, SCRATCH = kPairEpiWarps * kBoxBytes, MAX_STAGES = 8;
+  static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); X
     uint32_t bn;
@@ -406,13 +405,15 @@ struct RowsOp {
     double scale;
     const uint32_t *maxima;
     T *out;                  // the piece's first row
+    int boxes;               // out's rows are 16-byte aligned: `map` stores them
+    CUtensorMap map;
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
     return {(int32_t)((i / p.nt) * 256), (int32_t)((i % p.nt) * p.bn), 0, p.kblocks, 0};
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums, uint8_t *,
-                                                  uint32_t rank) {
+  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums,
+                                                  uint8_t *scratch, uint32_t rank) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t i = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
     double f = p.scale * (double)grad_unit(p.maxima[MAX_GRAD]) / kGradScale;
@@ -424,33 +425,37 @@ struct RowsOp {
     if (CHUNK) sums.template total<CHUNK + !CHUNK>(half * cols, w.kblocks, s);
     else tmem = sums.acquire() + half * cols;
     T *row = p.out + (uint64_t)i * p.dims;
-    const bool vec = p.dims % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+    BoxStore box{scratch + warp * kBoxBytes};
+    constexpr uint32_t BOX = 128 / sizeof(T), V = 16 / sizeof(T);   // values of a box row, of a chunk
 #pragma unroll
     for (uint32_t c = 0; c < 4; c++) {
-      const uint32_t c0 = c * 32, d0 = (uint32_t)w.b_row + half * cols + c0;
-      if (c0 >= cols || d0 >= p.dims) break;
+      const uint32_t d0 = (uint32_t)w.b_row + half * cols + c * 32;
+      if (c * 32 >= cols || d0 >= p.dims || i - lane >= p.rows) break;
       uint32_t r[32];
       if (CHUNK) {
 #pragma unroll
         for (int j = 0; j < 32; j++) r[j] = __float_as_uint(s[c][j]);
       } else {
-        sums.load(tmem + c0, r);
+        sums.load(tmem + c * 32, r);
       }
-      if (i >= p.rows) continue;
-      constexpr int V = 16 / sizeof(T);
+      const uint32_t at = c * 32 % BOX;     // of the box's values
+      if (p.boxes && at == 0) box.reuse();
 #pragma unroll
-      for (int j = 0; j < 32; j += V) {
-        alignas(16) T v[V];
+      for (uint32_t j = 0; j < 32; j += V) {
+        alignas(16) T o[V];
 #pragma unroll
-        for (int u = 0; u < V; u++) v[u] = from_float<T>(__uint_as_float(r[j + u]) * factor);
-        if (vec) {
-          if (d0 + j < p.dims) *reinterpret_cast<uint4 *>(row + d0 + j) = *reinterpret_cast<uint4 *>(v);
-        } else {
+        for (uint32_t u = 0; u < V; u++) o[u] = from_float<T>(__uint_as_float(r[j + u]) * factor);
+        if (p.boxes) {
+          box.put((at + j) / V, *reinterpret_cast<uint4 *>(o));
+        } else if (i < p.rows) {
 #pragma unroll
-          for (int u = 0; u < V; u++)
-            if (d0 + j + u < p.dims) row[d0 + j + u] = v[u];
+          for (uint32_t u = 0; u < V; u++)
+            if (d0 + j + u < p.dims) row[d0 + j + u] = o[u];
         }
       }
+      // the last 32 values of a box, or of the row
+      if (p.boxes && (at + 32 == BOX || d0 + 32 >= p.dims))
+        box.store(&p.map, (int32_t)((d0 - at) * (sizeof(T) / 2)), (int32_t)(i - lane));   // (in 16-bit values)
     }
     if (!CHUNK) sums.release();
   }
@@ -478,19 +483,23 @@ __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t 
                                                     double scale, const uint32_t *maxima, const double *total,
                                                     const T *rows, uint64_t stride, const int64_t *targets,
                                                     uint64_t nrows, T *out) {
-  const uint64_t n = (uint64_t)nq * dims;
+  const uint32_t q = blockIdx.x, ld = (dims + 3) / 4 * 4;
+  const uint64_t plane = (uint64_t)nq * ld;
   const double f = scale * (double)grad_unit(maxima[MAX_GRAD]) / kGradScale;
   const float factor = (float)f;
   const float undo = PLANES == 2 ? undo_scale(maxima[MAX_ROWS]) : 1.0f;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-    const uint32_t q = (uint32_t)(i / dims);
-    const int64_t t = targets[q];
+  const int64_t t = targets[q];
+  const bool kept = has_target(t, nrows);
+  const float left = kept ? -(float)total[q] : 0.0f;
+  const T *row = rows + (kept ? (uint64_t)t * stride : 0);
+  for (uint32_t d = threadIdx.x; d < dims; d += blockDim.x) {
     float v = 0.0f;
-    if (has_target(t, nrows)) {
-      for (uint32_t k = 0; k < splits; k++) v += part[k * n + i];
-      v = fmaf(-(float)total[q], to_float(rows[(uint64_t)t * stride + (i - (uint64_t)q * dims)]), v * undo) * factor;
+    if (kept) {
+      const float *at = part + (uint64_t)q * ld + d;
+      for (uint32_t k = 0; k < splits; k++) v += at[k * plane];
+      v = fmaf(left, to_float(row[d]), v * undo) * factor;
     }
-    out[i] = from_float<T>(v);
+    out[(uint64_t)q * dims + d] = from_float<T>(v);
   }
 }
 
@@ -563,7 +572,7 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
       }
       if (best >= 0.9) break;
     }
-    p.dq = c.take((uint64_t)p.splits * nq * j.dims * 4);
+    p.dq = c.take((uint64_t)p.splits * nq * up(j.dims, 4) * 4);
   }
   p.total = c.off;
   return p;
@@ -687,9 +696,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   l.mt = (j.nq + 255) / 256;
   l.lse = j.lse;
   l.grad = j.grad;
-  l.g = g;
-  l.ldg = p.piece;
-  l.gplane = gplane;
+  map(l.g, g, p.piece, j.nq, p.piece, gplane, 32);
   l.gsum = reinterpret_cast<float *>(ws + p.gsum);
   double *gtotal = reinterpret_cast<double *>(ws + p.gtotal);
   for (uint64_t first = 0; first < j.nrows && e == cudaSuccess; first += p.piece) {
@@ -710,7 +717,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       a.nq = j.nq;
       a.dims = j.dims;
       a.add = first != 0;
-      a.part = dq;
+      maps = maps && encode_sums_map(&a.part, dq, j.dims, j.nq, p.splits, up(j.dims, 4) * 4);
       fold_sums<<<(j.nq + 7) / 8, 256, 0, st>>>(l.gsum, 2 * l.nt, j.nq, a.add, gtotal);
       e = maps ? launch_pair<QOp>(a, a.mt * a.nt * a.splits, sms, st) : cudaErrorInvalidValue;
       launches += 2;
@@ -728,14 +735,17 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       a.scale = (double)j.scale;
       a.maxima = maxima;
       a.out = static_cast<T *>(j.drows) + first * j.dims;
+      a.boxes = (uint64_t)j.dims * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+      // (as 16-bit values, whatever T: a box is 128 bytes wide)
+      if (a.boxes)
+        maps = maps && encode_operand_map(&a.map, 2, a.out, j.dims * sizeof(T) / 2, n, j.dims * sizeof(T), 32);
       e = maps ? launch_pair<ROp>(a, a.mt * a.nt, sms, st) : cudaErrorInvalidValue;
       launches++;
     }
   }
   if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss gradient: %s", cudaGetErrorString(e));
   if (j.dqueries) {
-    const uint64_t n = (uint64_t)j.nq * j.dims;
-    join_queries<T, PLANES><<<(unsigned)std::min<uint64_t>((n + 255) / 256, 4736), 256, 0, st>>>(
+    join_queries<T, PLANES><<<j.nq, j.dims <= 128 ? 128 : 256, 0, st>>>(
         dq, p.splits, j.nq, j.dims, (double)j.scale, maxima, gtotal, w, j.row_stride, j.targets, j.nrows,
         static_cast<T *>(j.dqueries));
     launches++;

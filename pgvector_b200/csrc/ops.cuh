@@ -39,6 +39,9 @@ inline int op_launched(const char *what, unsigned long long kernels) {
 bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
                         uint64_t pitch, uint32_t box_rows);
 
+// FP32 sums [planes][outer][inner] in boxes of 32 values x 32 rows (shard.cu).
+bool encode_sums_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch);
+
 // SMs of the current device (a device's number never changes: asked once each).
 inline int op_sms() {
   static int known[64];

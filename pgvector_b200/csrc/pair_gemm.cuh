@@ -100,8 +100,10 @@ __device__ __forceinline__ uint32_t map_to_leader(uint32_t addr) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Relaxed: what it tells (tensor memory has been read, tcgen05.wait::ld) is in
+// registers; a release would wait for the epilogue's stores to memory as well.
 __device__ __forceinline__ void remote_arrive(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // A tile into this CTA's dst; completes on the leader's barrier (a cluster address).
 __device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
@@ -125,6 +127,58 @@ __device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volati
     }
   }
 }
+
+// A warp's way out to memory: 32 rows of 128 bytes, a row a lane, put into
+// shared memory in the 128-byte swizzle (each 16-byte chunk once: no bank
+// conflicts) and stored as one box by the TMA, whole lines at a time. Rows and
+// columns past the tensor's ends are left out by the TMA.
+constexpr int kBoxBytes = 32 * 128;
+struct BoxStore {
+  uint8_t *box;
+  // Before the box is filled again: what was stored from it has been read.
+  __device__ __forceinline__ void reuse() {
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+  }
+  __device__ __forceinline__ void put(uint32_t chunk, uint4 v) {
+    const uint32_t lane = threadIdx.x & 31;
+    *reinterpret_cast<uint4 *>(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = v;
+  }
+  __device__ __forceinline__ void store(const CUtensorMap *map, int32_t x, int32_t y) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                       reinterpret_cast<uint64_t>(map)),
+                   "r"(x), "r"(y), "r"(smem_u32(box))
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+  // FP32 into a plane, stored or added.
+  __device__ __forceinline__ void store_sums(const CUtensorMap *map, int32_t x, int32_t y, int32_t z, bool add) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      if (add)
+        asm volatile(
+            "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                reinterpret_cast<uint64_t>(map)),
+            "r"(x), "r"(y), "r"(z), "r"(smem_u32(box))
+            : "memory");
+      else
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                         reinterpret_cast<uint64_t>(map)),
+                     "r"(x), "r"(y), "r"(z), "r"(smem_u32(box))
+                     : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+  static __device__ __forceinline__ void finish() {
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+};
 
 // What an epilogue warp needs of the loop: the sums of one accumulator after
 // another. `ok` stays false once a wait has run out.
@@ -187,7 +241,8 @@ struct PairSums {
   }
 };
 
-// The shared memory of an operator's loop: stages of (A planes, B planes), then barriers.
+// The shared memory of an operator's loop: stages of (A planes, B planes), the
+// epilogue's scratch, barriers.
 template <class Op>
 struct PairShape {
   static constexpr int A_BYTES = Op::PLANES * kPairTileBytes;
@@ -217,7 +272,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t b_bytes = args.bn * 64;                 // bn / 2 rows (or columns) of 128 bytes each K block
   const uint32_t stage_bytes = Shape::stage(b_bytes);
   const uint32_t stages = Shape::stages(b_bytes);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + stages * stage_bytes);
+  uint8_t *scratch = smem + stages * stage_bytes;        // 1,024-byte aligned
+  uint64_t *full = reinterpret_cast<uint64_t *>(scratch + Op::SCRATCH);
   uint64_t *empty = full + MAXS;
   uint64_t *tfull = empty + MAXS;
   uint64_t *tempty = tfull + 2;
@@ -225,7 +281,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile uint32_t *abort = tmem_slot + 1;
   static_assert((2 * MAXS + 5) * 8 + 8 <= Shape::BAR_BYTES, "barriers");
-  uint8_t *scratch = reinterpret_cast<uint8_t *>(full) + Shape::BAR_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
@@ -258,14 +313,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   if (warp == 8) {
     if (lane == 0) {
-      uint32_t it = 0;
+      uint32_t s = 0, round = 0;
       bool ok = true;
       for (uint32_t i = cluster; i < items && ok; i += clusters) {
         const PairItem w = Op::item(args, i);
         const int32_t ar = w.a_row + (int32_t)rank * 128, br = w.b_row + (int32_t)(rank * (args.bn / 2));
-        for (uint32_t kb = 0; kb < w.kblocks; kb++, it++) {
-          const uint32_t s = it % stages;
-          if (!pair_wait(empty + s, ((it / stages) & 1) ^ 1, abort)) {
+        for (uint32_t kb = 0; kb < w.kblocks; kb++) {
+          if (!pair_wait(empty + s, (round & 1) ^ 1, abort)) {
             ok = false;
             break;
           }
@@ -288,6 +342,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               pair_load(b + p * b_bytes, &args.b[p], k, br, bar);
             }
           }
+          if (++s == stages) {
+            s = 0;
+            round++;
+          }
         }
       }
     }
@@ -296,19 +354,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = pair_idesc<Op::KIND, Op::A_MN, Op::B_MN>(args.bn);
       constexpr uint32_t A_STEP = Op::A_MN ? 2048 : 32, B_STEP = Op::B_MN ? 2048 : 32;
-      uint32_t it = 0, acc = 0;
+      uint32_t s = 0, round = 0, acc = 0;
       bool ok = true;
       for (uint32_t i = cluster; i < items && ok; i += clusters) {
         const PairItem w = Op::item(args, i);
-        for (uint32_t kb = 0; kb < w.kblocks; kb++, it++) {
+        for (uint32_t kb = 0; kb < w.kblocks; kb++) {
           const bool first = Op::CHUNK ? kb % (Op::CHUNK + !Op::CHUNK) == 0 : kb == 0;
           const bool last = kb + 1 == w.kblocks || (Op::CHUNK && (kb + 1) % (Op::CHUNK + !Op::CHUNK) == 0);
           if (first && !pair_wait(tempty + (acc & 1), ((acc >> 1) & 1) ^ 1, abort)) {
             ok = false;
             break;
           }
-          const uint32_t s = it % stages;
-          if (!pair_wait(full + s, (it / stages) & 1, abort)) {
+          if (!pair_wait(full + s, round & 1, abort)) {
             ok = false;
             break;
           }
@@ -336,6 +393,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             pair_commit(tfull + (acc & 1));
             acc++;
           }
+          if (++s == stages) {
+            s = 0;
+            round++;
+          }
         }
       }
       // the MMAs issued have ended, and the loads in flight have landed, before anything is freed
@@ -356,6 +417,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else {
     PairSums sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
     for (uint32_t i = cluster; i < items; i += clusters) Op::epilogue(args, Op::item(args, i), sums, scratch, rank);
+    BoxStore::finish();
   }
   tc_fence_before();
   __syncthreads();

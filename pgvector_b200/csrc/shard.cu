@@ -446,6 +446,19 @@ bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint
   return bytes == 1 ? encode_u8_seg_map(map, base, inner, outer, pitch, box_rows)
                     : encode_f16_map(map, base, inner, outer, pitch, box_rows);
 }
+// FP32 sums [planes][outer][inner], pitch bytes a row, written and added to in
+// swizzled boxes of 32 values x 32 rows of one plane.
+bool encode_sums_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {inner, outer, planes};
+  cuuint64_t strides[2] = {pitch, pitch * outer};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
 }  // namespace annb200
 
 extern "C" const char *AnnB200LastError(void) { return g_error.c_str(); }
