@@ -17,6 +17,7 @@
 // rows and, in the gradient, queries one e an array, since their sums run over
 // rows and queries; in the forward call one a query.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -154,13 +155,31 @@ __global__ void __launch_bounds__(256) pack_rows(const T *x, uint64_t stride, ui
 
 // ---------------------------------------------------------------- logits
 
+// Two values rounded to O, packed, and as FP32.
+template <typename O> __device__ __forceinline__ uint32_t round2(f32x2 v, f32x2 &kept);
+template <> __device__ __forceinline__ uint32_t round2<__nv_bfloat16>(f32x2 v, f32x2 &kept) {
+  float a, b;
+  unpack2(v, a, b);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const uint32_t u = *reinterpret_cast<const uint32_t *>(&h);
+  kept = pack2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  return u;
+}
+template <> __device__ __forceinline__ uint32_t round2<__half>(f32x2 v, f32x2 &kept) {
+  float a, b;
+  unpack2(v, a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  kept = pack2(__low2float(h), __high2float(h));
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // Tiles of 256 queries x 256 rows. GRAD: G of a piece; else the partial sums.
 template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
 struct LogitsOp {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? kPairEpiWarps * kBoxBytes : 0, MAX_STAGES = 8;
-  static constexpr int CHUNK = PLANES == 2 ? 1 : 4;
+  static constexpr int CHUNK = PLANES == 2 ? 2 : 6;   // 24 steps of the tensor cores
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];
     uint32_t bn;
@@ -182,120 +201,167 @@ struct LogitsOp {
     const uint32_t n = i / p.mt, m = i % p.mt;   // a row tile against all queries before the next
     return {(int32_t)(p.q0 + m * 256), (int32_t)(p.first + (uint64_t)n * 256), 0, p.kblocks, n};
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums,
-                                                  uint8_t *scratch, uint32_t rank) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
-    const uint32_t q = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
-    const bool valid = q < p.nq;
-    const bool any = __any_sync(0xffffffffu, valid);
-    float k = 0.0f;
-    int64_t tgt = -1;
-    float lse2 = 0.0f, g = 0.0f;
-    bool kept = false;
-    if (valid) {
-      double s = p.scale2;
-      if (PLANES == 2) s *= (double)p.xscale[q] * (double)undo_scale(p.maxima[MAX_ROWS]);
-      k = (float)s;
-      tgt = p.targets[q];
-      if (GRAD) {
-        kept = has_target(tgt, p.nrows);
-        lse2 = p.lse[q] * kLog2e;
-        g = kept ? (p.grad ? p.grad[q] : 1.0f) / grad_unit(p.maxima[MAX_GRAD]) * kGradScale : 0.0f;
-      }
+  // What an item's epilogue reads of its query, loaded an item ahead.
+  struct Row {
+    int64_t target;
+    float lse, grad, xscale;
+  };
+  static __device__ __forceinline__ uint32_t query_of(const PairItem &w, uint32_t rank) {
+    return (uint32_t)w.a_row + rank * 128 + ((threadIdx.x >> 5) & 3) * 32 + (threadIdx.x & 31);
+  }
+  static __device__ __forceinline__ Row row_of(const Args &p, uint32_t i, uint32_t rank) {
+    Row r = {-1, 0.0f, 0.0f, 1.0f};
+    if (i >= items(p)) return r;
+    const uint32_t q = query_of(item(p, i), rank);
+    if (q >= p.nq) return r;
+    r.target = p.targets[q];
+    if (PLANES == 2) r.xscale = p.xscale[q];
+    if (GRAD) {
+      r.lse = p.lse[q];
+      r.grad = p.grad ? p.grad[q] : 1.0f;
     }
-    const int64_t col0 = (int64_t)w.b_row + half * 128;   // this thread's first row of W
-    const int64_t at = tgt - col0;                        // the target's column, if in [0, 128)
-    float v[4][32];
-    sums.template total<CHUNK>(half * 128, w.kblocks, v);
-    if (any) {
-      float m = -INFINITY, s = 0.0f;   // of this thread's 128 columns
-      const int64_t left = (int64_t)p.nrows - col0;       // columns that are rows of W
-      const bool hit = __any_sync(0xffffffffu, valid && at >= 0 && at < 128);
+    return r;
+  }
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+                                                  uint32_t cluster, uint32_t clusters) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
+    const double scale2 = PLANES == 2 ? p.scale2 * (double)undo_scale(p.maxima[MAX_ROWS]) : p.scale2;
+    const float unit = GRAD ? grad_unit(p.maxima[MAX_GRAD]) : 1.0f;
+    BoxStore box{scratch + warp * kBoxBytes};
+    Row next = row_of(p, cluster, rank);
+    for (uint32_t i = cluster; i < items(p); i += clusters) {
+      const PairItem w = item(p, i);
+      const Row row = next;
+      next = row_of(p, i + clusters, rank);
+      const uint32_t q = query_of(w, rank);
+      const bool valid = q < p.nq;
+      const int64_t col0 = (int64_t)w.b_row + half * 128;   // this thread's first row of W
+      f32x2 v[64];
+      sums.template total<CHUNK, 4>(half * 128, w.kblocks, v);
+      if (!__any_sync(0xffffffffu, valid)) continue;
+      float k = PLANES == 2 ? (float)(scale2 * (double)row.xscale) : (float)scale2;
+      if (k == 0.0f) k = FLT_MIN;   // (0 would make NaNs of the infinities that stand for no column)
+      const int64_t left = (int64_t)p.nrows - col0;         // columns that are rows of W
+      // the target's column, 128 where it is not here
+      const int64_t rel = row.target - col0;
+      const int at = valid && rel >= 0 && rel < 128 ? (int)rel : 128;
+      const bool hit = __any_sync(0xffffffffu, at < 128);
+      float s = 0.0f;                                       // of this thread's 128 columns
       if (!GRAD) {
-        // in base 2; columns past the rows count for nothing
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[c][j] *= k;
         if (hit) {
           float t = 0.0f;
 #pragma unroll
-          for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int j = 0; j < 32; j++) t = (int)at == c * 32 + j ? v[c][j] : t;
-          if (valid && at >= 0 && at < 128) p.tlogit[q] = t;
+          for (int j = 0; j < 64; j++) {
+            float a, b;
+            unpack2(v[j], a, b);
+            t = at == 2 * j ? a : (at == 2 * j + 1 ? b : t);
+          }
+          if (at < 128) p.tlogit[q] = t * k;
         }
-        if (left < 128) {
+        if (left < 128) {   // columns past the rows count for nothing
+          const float none = k < 0.0f ? INFINITY : -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[c][j] = c * 32 + j < (int)left ? v[c][j] : -INFINITY;
+          for (int j = 0; j < 64; j++) {
+            float a, b;
+            unpack2(v[j], a, b);
+            v[j] = pack2(2 * j < (int)left ? a : none, 2 * j + 1 < (int)left ? b : none);
+          }
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // the largest logit in base 2
+        float top[4];
+        const float start = k < 0.0f ? INFINITY : -INFINITY;
+        top[0] = top[1] = top[2] = top[3] = start;
+        if (k < 0.0f) {
 #pragma unroll
-        for (int c = 0; c < 4; c++)
+          for (int j = 0; j < 64; j++) {
+            float a, b;
+            unpack2(v[j], a, b);
+            top[j & 3] = min3(top[j & 3], a, b);
+          }
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; j++) top[j & 3] = fmaxf(top[j & 3], v[c][j]);
-        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          for (int j = 0; j < 64; j++) {
+            float a, b;
+            unpack2(v[j], a, b);
+            top[j & 3] = max3(top[j & 3], a, b);
+          }
+        }
+        const float most = k < 0.0f ? fminf(fminf(top[0], top[1]), fminf(top[2], top[3]))
+                                    : fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float m = left <= 0 ? -INFINITY : most * k;
         const float base = m == -INFINITY ? 0.0f : m;
-        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const f32x2 kk = pack2(k, k), bb = pack2(-base, -base);
+        f32x2 e[4] = {};
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int j = 0; j < 32; j++) e[j & 3] += exp2_approx(v[c][j] - base);
-        s = (e[0] + e[1]) + (e[2] + e[3]);
+        for (int j = 0; j < 64; j++) {
+          float a, b;
+          unpack2(fma2(v[j], kk, bb), a, b);
+          e[j & 3] = add2(e[j & 3], pack2(exp2_approx(a), exp2_approx(b)));
+        }
+        float a, b;
+        unpack2(add2(add2(e[0], e[1]), add2(e[2], e[3])), a, b);
+        s = a + b;
+        if (left <= 0) s = 0.0f;
+        if (valid) p.part[(uint64_t)(q - p.q0) * (2 * p.nt) + 2 * w.index + half] = make_float2(m, s);
       } else {
         // G; columns past the rows go to the buffer's end, which is not read
+        const bool kept = valid && has_target(row.target, p.nrows);
+        const float lse2 = row.lse * kLog2e, g = kept ? row.grad / unit * kGradScale : 0.0f;
+        const f32x2 kk = pack2(k, k), zz = pack2(-lse2, -lse2), gg = pack2(g, g);
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[c][j] = exp2_approx(fmaf(v[c][j], k, -lse2));
+        for (int j = 0; j < 64; j++) {
+          float a, b;
+          unpack2(fma2(v[j], kk, zz), a, b);
+          v[j] = pack2(exp2_approx(a), exp2_approx(b));
+        }
         if (hit) {
 #pragma unroll
-          for (int c = 0; c < 4; c++)
+          for (int j = 0; j < 64; j++)
+            v[j] = add2(v[j], pack2(at == 2 * j ? -1.0f : 0.0f, at == 2 * j + 1 ? -1.0f : 0.0f));
+        }
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[c][j] -= at == c * 32 + j ? 1.0f : 0.0f;
+        for (int j = 0; j < 64; j++) v[j] = mul2(v[j], gg);
+        if (!kept) {        // (not 0 times what the query holds)
+#pragma unroll
+          for (int j = 0; j < 64; j++) v[j] = 0;
         }
         if (left < 128) {
 #pragma unroll
-          for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[c][j] = c * 32 + j < (int)left ? v[c][j] : 0.0f;
+          for (int j = 0; j < 64; j++) {
+            float a, b;
+            unpack2(v[j], a, b);
+            v[j] = pack2(2 * j < (int)left ? a : 0.0f, 2 * j + 1 < (int)left ? b : 0.0f);
+          }
         }
-        const BoxStore box{scratch + warp * kBoxBytes};
         const int32_t x = (int32_t)(col0 - (int64_t)p.first), y = (int32_t)(q - lane);
+        f32x2 sum[2] = {};
         // of a plane: the values it keeps, taken off v, and their sum
-        auto plane = [&](const CUtensorMap *map, bool last) {
-          float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int plane = 0; plane < PLANES; plane++) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            BoxStore(box).reuse();
+            box.reuse();
 #pragma unroll
             for (int c = 0; c < 8; c++) {
-              alignas(16) O o[8];
+              uint32_t o[4];
 #pragma unroll
-              for (int j = 0; j < 8; j++) {
-                float &f = v[2 * h + c / 4][(c & 3) * 8 + j];
-                o[j] = from_float<O>(f);
-                const float kept_value = to_float(o[j]);
-                sum[j & 1] += kept_value;
-                if (!last) f -= kept_value;
+              for (int j = 0; j < 4; j++) {
+                f32x2 &f = v[32 * h + 4 * c + j];
+                f32x2 kept_values;
+                o[j] = round2<O>(f, kept_values);
+                sum[j & 1] = add2(sum[j & 1], kept_values);
+                if (plane + 1 < PLANES) f = fma2(kept_values, pack2(-1.0f, -1.0f), f);
               }
-              BoxStore(box).put(c, *reinterpret_cast<uint4 *>(o));
+              box.put(c, make_uint4(o[0], o[1], o[2], o[3]));
             }
-            BoxStore(box).store(map, x + h * 64, y);
+            box.store(&p.g[plane], x + h * 64, y);
           }
-          s += sum[0] + sum[1];
-        };
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[c][j] = kept ? v[c][j] * g : 0.0f;
-        plane(&p.g[0], PLANES == 1);
-        if (PLANES == 2) plane(&p.g[PLANES - 1], true);
+        }
+        float a, b;
+        unpack2(add2(sum[0], sum[1]), a, b);
+        s = a + b;
+        if (valid) p.gsum[(uint64_t)q * (2 * p.nt) + 2 * w.index + half] = s;
       }
-      if (GRAD && valid) p.gsum[(uint64_t)q * (2 * p.nt) + 2 * w.index + half] = s;
-      if (!GRAD && valid) p.part[(uint64_t)(q - p.q0) * (2 * p.nt) + 2 * w.index + half] = make_float2(m, s);
     }
   }
 };
@@ -359,15 +425,19 @@ struct QueriesOp {
     const uint32_t k1 = (uint32_t)((uint64_t)p.kblocks * (s + 1) / p.splits);
     return {(int32_t)((t / p.nt) * 256), (int32_t)((t % p.nt) * p.bn), (int32_t)(k0 * 64), k1 - k0, s};
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums,
-                                                  uint8_t *scratch, uint32_t rank) {
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+                                                  uint32_t cluster, uint32_t clusters) {
+    for (uint32_t i = cluster; i < items(p); i += clusters) tile(p, item(p, i), sums, scratch, rank);
+  }
+  static __device__ __forceinline__ void tile(const Args &p, const PairItem &w, PairSums &sums, uint8_t *scratch,
+                                              uint32_t rank) {
     if (w.kblocks == 0) return;   // (a short last piece; its partial stays)
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t q = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
     const uint32_t cols = p.bn / 2;
-    float v[4][32];
+    f32x2 v[64];
     uint32_t tmem = 0;
-    if (CHUNK) sums.template total<CHUNK + !CHUNK>(half * cols, w.kblocks, v);
+    if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
     else tmem = sums.acquire() + half * cols;
     BoxStore box{scratch + warp * kBoxBytes};
 #pragma unroll
@@ -377,7 +447,12 @@ struct QueriesOp {
       uint32_t r[32];
       if (CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) r[j] = __float_as_uint(v[c][j]);
+        for (int j = 0; j < 16; j++) {
+          float a, b;
+          unpack2(v[16 * c + j], a, b);
+          r[2 * j] = __float_as_uint(a);
+          r[2 * j + 1] = __float_as_uint(b);
+        }
       } else {
         sums.load(tmem + c * 32, r);
       }
@@ -412,17 +487,21 @@ struct RowsOp {
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
     return {(int32_t)((i / p.nt) * 256), (int32_t)((i % p.nt) * p.bn), 0, p.kblocks, 0};
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, const PairItem &w, PairSums &sums,
-                                                  uint8_t *scratch, uint32_t rank) {
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+                                                  uint32_t cluster, uint32_t clusters) {
+    for (uint32_t i = cluster; i < items(p); i += clusters) tile(p, item(p, i), sums, scratch, rank);
+  }
+  static __device__ __forceinline__ void tile(const Args &p, const PairItem &w, PairSums &sums, uint8_t *scratch,
+                                              uint32_t rank) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t i = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
     double f = p.scale * (double)grad_unit(p.maxima[MAX_GRAD]) / kGradScale;
     if (PLANES == 2) f *= (double)undo_scale(p.maxima[MAX_QUERIES]);
     const float factor = (float)f;
     const uint32_t cols = p.bn / 2;
-    float s[4][32];
+    f32x2 v[64];
     uint32_t tmem = 0;
-    if (CHUNK) sums.template total<CHUNK + !CHUNK>(half * cols, w.kblocks, s);
+    if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
     else tmem = sums.acquire() + half * cols;
     T *row = p.out + (uint64_t)i * p.dims;
     BoxStore box{scratch + warp * kBoxBytes};
@@ -434,7 +513,12 @@ struct RowsOp {
       uint32_t r[32];
       if (CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) r[j] = __float_as_uint(s[c][j]);
+        for (int j = 0; j < 16; j++) {
+          float a, b;
+          unpack2(v[16 * c + j], a, b);
+          r[2 * j] = __float_as_uint(a);
+          r[2 * j + 1] = __float_as_uint(b);
+        }
       } else {
         sums.load(tmem + c * 32, r);
       }

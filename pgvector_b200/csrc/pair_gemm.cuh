@@ -203,11 +203,9 @@ struct PairSums {
   }
   // N x 32 columns from `at` on, of the item's whole K: its chunks, added up.
   template <int CHUNK, int N>
-  __device__ __forceinline__ void total(uint32_t at, uint32_t kblocks, float (&v)[N][32]) {
+  __device__ __forceinline__ void total(uint32_t at, uint32_t kblocks, f32x2 (&v)[16 * N]) {
 #pragma unroll
-    for (int c = 0; c < N; c++)
-#pragma unroll
-      for (int j = 0; j < 32; j++) v[c][j] = 0.0f;
+    for (int j = 0; j < 16 * N; j++) v[j] = 0;
 #pragma unroll 1
     for (uint32_t kb = 0; kb < kblocks; kb += CHUNK) {
       const uint32_t addr = acquire() + at;
@@ -218,16 +216,16 @@ struct PairSums {
           TMEM_LD32(addr + c * 32, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[c][j] += __uint_as_float(r[j]);
+          for (int j = 0; j < 16; j++)
+            v[16 * c + j] = add2(v[16 * c + j], pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
         }
       }
       release();
     }
-    const float poison = ok ? 0.0f : __uint_as_float(0x7fc00000u);
+    if (!ok) {
 #pragma unroll
-    for (int c = 0; c < N; c++)
-#pragma unroll
-      for (int j = 0; j < 32; j++) v[c][j] += poison;
+      for (int j = 0; j < 16 * N; j++) v[j] = pack2(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u));
+    }
   }
   // 32 columns of this thread's row.
   __device__ __forceinline__ void load(uint32_t addr, uint32_t (&r)[32]) {
@@ -259,7 +257,7 @@ struct PairShape {
 // Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
 // sum; 0: the item's), Args with maps a[PLANES],
 // b[PLANES] and bn (columns of a tile), items(args), item(args, i),
-// epilogue(args, item, sums, scratch, rank).
+// epilogue(args, sums, scratch, rank, cluster, clusters): all of the cluster's items.
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_gemm(const __grid_constant__ typename Op::Args args) {
@@ -416,7 +414,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     __syncwarp();
   } else {
     PairSums sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
-    for (uint32_t i = cluster; i < items; i += clusters) Op::epilogue(args, Op::item(args, i), sums, scratch, rank);
+    Op::epilogue(args, sums, scratch, rank, cluster, clusters);
     BoxStore::finish();
   }
   tc_fence_before();
