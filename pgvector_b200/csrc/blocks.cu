@@ -1,16 +1,25 @@
 // blocks.cu - E4M3 with one FP32 scale per block of 128: the quantizer and the
 // product of two operands in that form (AnnB200QuantizeBlocks,
 // AnnB200MatmulBlocks).
+//
+// The product has two kernels. With up to 4 rows in a (single queries) it is
+// bound by reading b once: a warp a few rows of b, CUDA cores. Above that the
+// tensor cores (pair_gemm.cuh), b's rows as the tile's 256 rows and a's as its
+// columns: a K block of 128 is one sum in tensor memory, which the epilogue
+// takes out, scales and adds up in FP32 registers while the next block's
+// products run.
 #include <cuda_fp8.h>
 
 #include <algorithm>
 
-#include "ops.cuh"
+#include "pair_gemm.cuh"
 
 namespace annb200 {
 namespace {
 
 constexpr uint32_t kBlock = 128;
+
+// ---------------------------------------------------------------- quantizer
 
 // A block's scale and its inverse from absmax's bits (integer order keeps a
 // NaN above everything): 448 / a, a at least 2^-100; 0 gives scale 1.
@@ -20,73 +29,370 @@ __device__ __forceinline__ float block_scale(uint32_t bits, float &inverse) {
   return __fdiv_rn(a, 448.0f);
 }
 
-__device__ __forceinline__ uint8_t e4m3_code(float v) {
-  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+// 8 values of a row from column c on (c % 8 == 0), zero past k. vec: rows are 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(const T *row, uint32_t c, uint32_t k, bool vec, float (&v)[8]) {
+  if (vec && c + 8 <= k) {
+    alignas(16) T t[8];
+#pragma unroll
+    for (int j = 0; j < (int)(8 * sizeof(T) / 16); j++)
+      reinterpret_cast<uint4 *>(t)[j] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + j);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = to_float(t[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = c + j < k ? to_float(row[c + j]) : 0.0f;
+  }
+}
+__device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) b = max(b, __float_as_uint(v[j]) & 0x7fffffffu);
+  return b;
+}
+// The codes of 8 values, rounded to nearest (ties to even) by the hardware's conversion.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inverse) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    w[j] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(v[2 * j], inverse), __fmul_rn(v[2 * j + 1], inverse)),
+                                    __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-// One block of the output grid a 1 x 128 or 128 x 128 block, 128 threads.
+// Blocks of 1 x 128: 16 lanes a block, 8 values a lane, read once and kept in
+// registers. Bound by memory: UNITS blocks a half warp are in flight.
+constexpr int kQuantUnits = 4;
 template <typename T>
-__global__ void __launch_bounds__(128) quantize(const T *x, uint64_t stride, uint64_t m, uint32_t k, uint32_t height,
-                                                uint8_t *codes, uint64_t code_stride, float *scales) {
-  const uint32_t kb = (k + kBlock - 1) / kBlock;
-  const uint64_t rb = blockIdx.x / kb;
-  const uint32_t b = (uint32_t)(blockIdx.x % kb);
-  const uint64_t r0 = rb * height, r1 = min(m, r0 + height);
-  const uint32_t c = b * kBlock + threadIdx.x;
+__global__ void __launch_bounds__(256) quantize_rows(const T *x, uint64_t stride, uint64_t blocks, uint32_t k,
+                                                     uint32_t kb, uint8_t *codes, uint64_t code_stride,
+                                                     float *scales) {
+  const uint32_t lane = threadIdx.x & 15;
+  const bool vec = stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const uint32_t k16 = (k + 15) / 16 * 16;
-  __shared__ uint32_t top[4];
+  const uint64_t u0 = ((uint64_t)blockIdx.x * 16 + threadIdx.x / 16) * kQuantUnits;
+  float v[kQuantUnits][8];
+  uint64_t row[kQuantUnits];
+  uint32_t col[kQuantUnits];
+  row[0] = blocks < 0x80000000ull ? (uint32_t)u0 / kb : u0 / kb;
+  uint32_t b = (uint32_t)(u0 - row[0] * kb);
+#pragma unroll
+  for (int u = 0; u < kQuantUnits; u++) {
+    if (u > 0) row[u] = row[u - 1];
+    if (b == kb) {
+      b = 0;
+      row[u]++;
+    }
+    col[u] = b++ * kBlock + lane * 8;
+    if (u0 + u < blocks) load8(x + row[u] * stride, col[u], k, vec, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantUnits; u++) {
+    const bool in = u0 + u < blocks;
+    uint32_t bits = in ? largest_bits(v[u]) : 0;
+#pragma unroll
+    for (int d = 8; d; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+    float inverse;
+    const float scale = block_scale(bits, inverse);
+    if (!in) continue;
+    if (lane == 0) scales[u0 + u] = scale;
+    if (col[u] < k16) *reinterpret_cast<uint2 *>(codes + row[u] * code_stride + col[u]) = codes8(v[u], inverse);
+  }
+}
+
+// Blocks of 128 x 128: a CTA a block, 8 rows x 8 values a thread in registers.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_square(const T *x, uint64_t stride, uint64_t m, uint32_t k, uint32_t kb,
+                                                       uint8_t *codes, uint64_t code_stride, float *scales) {
+  const uint32_t lane = threadIdx.x & 15;
+  const bool vec = stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const uint32_t k16 = (k + 15) / 16 * 16;
+  const uint64_t r0 = (uint64_t)(blockIdx.x / kb) * kBlock + threadIdx.x / 16;
+  const uint32_t c = blockIdx.x % kb * kBlock + lane * 8;
+  float v[8][8];
   uint32_t bits = 0;
-  if (c < k)
-    for (uint64_t r = r0; r < r1; r++) bits = max(bits, __float_as_uint(to_float(x[r * stride + c])) & 0x7fffffffu);
+#pragma unroll
+  for (int u = 0; u < 8; u++) {
+    if (r0 + 16 * u < m) {
+      load8(x + (r0 + 16 * u) * stride, c, k, vec, v[u]);
+      bits = max(bits, largest_bits(v[u]));
+    }
+  }
+  __shared__ uint32_t top[8];
   bits = __reduce_max_sync(0xffffffffu, bits);
   if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = bits;
   __syncthreads();
-  bits = max(max(top[0], top[1]), max(top[2], top[3]));
+  bits = 0;
+#pragma unroll
+  for (int u = 0; u < 8; u++) bits = max(bits, top[u]);
   float inverse;
   const float scale = block_scale(bits, inverse);
-  if (threadIdx.x == 0) scales[rb * kb + b] = scale;
-  if (c < k16)
-    for (uint64_t r = r0; r < r1; r++)
-      codes[r * code_stride + c] = c < k ? e4m3_code(__fmul_rn(to_float(x[r * stride + c]), inverse)) : 0;
+  if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+  if (c >= k16) return;
+#pragma unroll
+  for (int u = 0; u < 8; u++)
+    if (r0 + 16 * u < m)
+      *reinterpret_cast<uint2 *>(codes + (r0 + 16 * u) * code_stride + c) = codes8(v[u], inverse);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
-    matmul(const uint8_t *a, uint64_t a_stride, const float *a_scales, uint32_t a_shift, const uint8_t *b,
-           uint64_t b_stride, const float *b_scales, uint32_t b_shift, uint64_t m, uint64_t n, uint32_t k, T *out,
-           uint64_t out_stride) {
-  __shared__ float as[16][68], bs[16][68];
-  const uint64_t m0 = (uint64_t)blockIdx.y * 64, n0 = (uint64_t)blockIdx.x * 64;
-  const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
+void launch_quantize(const T *x, uint64_t stride, uint64_t m, uint32_t k, bool square, uint8_t *codes,
+                     uint64_t code_stride, float *scales, cudaStream_t st) {
   const uint32_t kb = (k + kBlock - 1) / kBlock;
-  float sum[4][4] = {};
-  for (uint32_t blk = 0; blk < kb; blk++) {
-    float acc[4][4] = {};
-    const uint32_t kend = min(k, (blk + 1) * kBlock);
-    for (uint32_t k0 = blk * kBlock; k0 < kend; k0 += 16) {
-      for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-        const int r = i / 16, c = i % 16;
-        as[c][r] = m0 + r < m && k0 + c < kend ? e4m3_value(a[(m0 + r) * a_stride + k0 + c]) : 0.0f;
-        bs[c][r] = n0 + r < n && k0 + c < kend ? e4m3_value(b[(n0 + r) * b_stride + k0 + c]) : 0.0f;
-      }
-      __syncthreads();
-      for (int c = 0; c < 16; c++)
-        for (int i = 0; i < 4; i++)
-          for (int j = 0; j < 4; j++) acc[i][j] = fmaf(as[c][tm * 4 + i], bs[c][tn * 4 + j], acc[i][j]);
-      __syncthreads();
-    }
-    for (int i = 0; i < 4; i++)
-      for (int j = 0; j < 4; j++) {
-        const uint64_t r = m0 + tm * 4 + i, c = n0 + tn * 4 + j;
-        if (r < m && c < n)
-          sum[i][j] += acc[i][j] * (a_scales[(r >> a_shift) * kb + blk] * b_scales[(c >> b_shift) * kb + blk]);
-      }
+  if (square) {
+    quantize_square<<<(unsigned)((m + kBlock - 1) / kBlock * kb), 256, 0, st>>>(x, stride, m, k, kb, codes,
+                                                                               code_stride, scales);
+  } else {
+    const uint64_t blocks = m * kb;
+    quantize_rows<<<(unsigned)((blocks + 16 * kQuantUnits - 1) / (16 * kQuantUnits)), 256, 0, st>>>(
+        x, stride, blocks, k, kb, codes, code_stride, scales);
   }
-  for (int i = 0; i < 4; i++)
+}
+
+// ---------------------------------------------------------------- product, few rows of a
+
+struct Operands {
+  const uint8_t *a, *b;
+  uint64_t a_stride, b_stride;
+  const float *a_scales, *b_scales;
+  uint32_t a_shift, b_shift;   // 7 for square blocks: rows / 128
+  uint64_t m, n;
+  uint32_t k, kb;
+  uint64_t out_stride;
+};
+
+// Four E4M3 codes -> two pairs of FP32 (through FP16, which holds them all).
+__device__ __forceinline__ void decode4(uint32_t w, f32x2 &lo, f32x2 &hi) {
+  const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+  const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+  lo = pack2(x.x, x.y);
+  hi = pack2(y.x, y.y);
+}
+// 16 codes of a row from column c on; those past k are zero.
+__device__ __forceinline__ uint4 load16(const uint8_t *row, uint32_t c, uint32_t k) {
+  if (c >= k) return make_uint4(0, 0, 0, 0);
+  uint4 w = __ldg(reinterpret_cast<const uint4 *>(row + c));
+  if (c + 16 > k) {
+    uint32_t *p = reinterpret_cast<uint32_t *>(&w);
+#pragma unroll
     for (int j = 0; j < 4; j++) {
-      const uint64_t r = m0 + tm * 4 + i, c = n0 + tn * 4 + j;
-      if (r < m && c < n) out[r * out_stride + c] = from_float<T>(sum[i][j]);
+      const int left = (int)(k - c) - 4 * j;
+      if (left < 4) p[j] = left <= 0 ? 0u : p[j] & ((1u << (8 * left)) - 1u);
     }
+  }
+  return w;
+}
+
+// A warp kFewRows rows of b against all M rows of a: 16 codes a lane, 512 of K
+// a step (8 lanes a block), each lane's products times its block's scales into
+// its own FP32 sums; the lanes' sums joined at the end.
+constexpr int kFewRows = 4;
+template <int M, typename T>
+__global__ void __launch_bounds__(256, M == 1 ? 3 : 2) matmul_few(const Operands p, T *out) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t n0 = ((uint64_t)blockIdx.x * 8 + warp) * kFewRows;
+  if (n0 >= p.n) return;
+  float sum[kFewRows][M] = {};
+  const uint8_t *brow[kFewRows];
+  const float *bscale[kFewRows];
+#pragma unroll
+  for (int r = 0; r < kFewRows; r++) {
+    const uint64_t n = min(n0 + r, p.n - 1);
+    brow[r] = p.b + n * p.b_stride;
+    bscale[r] = p.b_scales + (n >> p.b_shift) * p.kb;
+  }
+#pragma unroll 2
+  for (uint32_t c = lane * 16; c < p.k; c += 512) {
+    uint4 wb[kFewRows];
+    float sb[kFewRows];
+#pragma unroll
+    for (int r = 0; r < kFewRows; r++) {
+      wb[r] = load16(brow[r], c, p.k);
+      sb[r] = __ldg(bscale[r] + c / kBlock);
+    }
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+      const uint64_t m = i < p.m ? i : p.m - 1;
+      const uint4 wa = load16(p.a + m * p.a_stride, c, p.k);
+      const float sa = __ldg(p.a_scales + (m >> p.a_shift) * p.kb + c / kBlock);
+      f32x2 av[8];
+      decode4(wa.x, av[0], av[1]);
+      decode4(wa.y, av[2], av[3]);
+      decode4(wa.z, av[4], av[5]);
+      decode4(wa.w, av[6], av[7]);
+#pragma unroll
+      for (int r = 0; r < kFewRows; r++) {
+        f32x2 bv[8];
+        decode4(wb[r].x, bv[0], bv[1]);
+        decode4(wb[r].y, bv[2], bv[3]);
+        decode4(wb[r].z, bv[4], bv[5]);
+        decode4(wb[r].w, bv[6], bv[7]);
+        f32x2 d[2] = {mul2(av[0], bv[0]), mul2(av[1], bv[1])};
+#pragma unroll
+        for (int j = 2; j < 8; j++) d[j & 1] = fma2(av[j], bv[j], d[j & 1]);
+        float x, y;
+        unpack2(add2(d[0], d[1]), x, y);
+        sum[r][i] = fmaf(x + y, sa * sb[r], sum[r][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kFewRows; r++)
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+      float s = sum[r][i];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (lane == 0 && n0 + r < p.n && i < p.m) out[(uint64_t)i * p.out_stride + n0 + r] = from_float<T>(s);
+    }
+}
+
+// ---------------------------------------------------------------- product, tensor cores
+
+// Tiles of 256 of b's rows (lanes) x 2 COLS of a's (columns, COLS a thread).
+// UNIFORM: b's scales are square, so a warp's rows share them and they join
+// a's in shared memory: one multiply-add a value instead of two operations.
+template <int COLS, bool UNIFORM, typename T>
+struct BlocksOp {
+  static constexpr PairKind KIND = PAIR_E4M3;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1;
+  static constexpr int AHEAD = 4;   // blocks whose scales are staged at a time
+  static constexpr int SCRATCH = 2 * AHEAD * 2 * COLS * 4;
+  struct Args {
+    CUtensorMap a[1], b[1];   // the tile's rows (the product's b) and columns (its a)
+    uint32_t bn;              // 2 COLS
+    uint32_t mt, nt;          // tiles of a's rows, of b's
+    Operands o;
+    T *out;
+  };
+  static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
+  static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
+    return {(int32_t)((i / p.mt) * 256), (int32_t)((i % p.mt) * p.bn), 0, p.o.kb, 0};
+  }
+  // Scales b0 .. b0 + 3 of a row of blocks (0 past the last).
+  static __device__ __forceinline__ float4 scales4(const float *row, uint32_t b0, uint32_t kb) {
+    if (b0 + 4 <= kb && (kb & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0)
+      return __ldg(reinterpret_cast<const float4 *>(row + b0));
+    float4 v;
+    v.x = b0 < kb ? __ldg(row + b0) : 0.0f;
+    v.y = b0 + 1 < kb ? __ldg(row + b0 + 1) : 0.0f;
+    v.z = b0 + 2 < kb ? __ldg(row + b0 + 2) : 0.0f;
+    v.w = b0 + 3 < kb ? __ldg(row + b0 + 3) : 0.0f;
+    return v;
+  }
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+                                                  uint32_t cluster, uint32_t clusters) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
+    float *stage = reinterpret_cast<float *>(scratch) + half * COLS;   // [2][AHEAD][2 COLS]
+    const Operands &o = p.o;
+    uint32_t group = 0;
+    for (uint32_t i = cluster; i < items(p); i += clusters) {
+      const PairItem w = item(p, i);
+      const uint64_t n = (uint64_t)w.a_row + rank * 128 + quad * 32 + lane;   // b's row
+      const uint64_t m0 = (uint64_t)w.b_row + half * COLS;                    // a's first row
+      const float *lane_scales = o.b_scales + (min(n, o.n - 1) >> o.b_shift) * o.kb;
+      // the half's four warps stage COLS rows' scales between them
+      const uint32_t mine = quad * 32 + lane;
+      const bool stages = mine < COLS;
+      const float *col_scales = o.a_scales + (min(m0 + mine, o.m - 1) >> o.a_shift) * o.kb;
+      f32x2 v[COLS / 2];
+#pragma unroll
+      for (int j = 0; j < COLS / 2; j++) v[j] = 0;
+      float4 sb = scales4(lane_scales, 0, o.kb), sa = stages ? scales4(col_scales, 0, o.kb) : make_float4(0, 0, 0, 0);
+      for (uint32_t b0 = 0; b0 < o.kb; b0 += AHEAD, group++) {
+        float *at = stage + (group & 1) * (AHEAD * 2 * COLS);
+        const float4 own = sb;
+        if (stages) {
+          at[mine] = UNIFORM ? sa.x * own.x : sa.x;
+          at[2 * COLS + mine] = UNIFORM ? sa.y * own.y : sa.y;
+          at[4 * COLS + mine] = UNIFORM ? sa.z * own.z : sa.z;
+          at[6 * COLS + mine] = UNIFORM ? sa.w * own.w : sa.w;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        if (b0 + AHEAD < o.kb) {   // the next group's, under this one's products
+          sb = scales4(lane_scales, b0 + AHEAD, o.kb);
+          if (stages) sa = scales4(col_scales, b0 + AHEAD, o.kb);
+        }
+#pragma unroll 1
+        for (uint32_t g = 0; g < AHEAD && b0 + g < o.kb; g++) {
+          const uint32_t addr = sums.acquire() + half * COLS;
+          const float *scale = at + g * 2 * COLS;
+          const float l = g == 0 ? own.x : (g == 1 ? own.y : (g == 2 ? own.z : own.w));
+          const f32x2 ls = pack2(l, l);
+          constexpr int STEP = COLS < 32 ? COLS : 32;
+#pragma unroll
+          for (int c = 0; c < COLS / STEP; c++) {
+            uint32_t r[STEP];
+            if (sums.ok) {
+              if constexpr (STEP == 32) TMEM_LD32(addr + c * 32, r);
+              else TMEM_LD16(addr, r);
+              tmem_ld_wait();
+            }
+            if (c + 1 == COLS / STEP) sums.release();
+#pragma unroll
+            for (int j = 0; j < STEP; j += 4) {
+              const float4 s4 = *reinterpret_cast<const float4 *>(scale + c * STEP + j);
+              f32x2 s0 = pack2(s4.x, s4.y), s1 = pack2(s4.z, s4.w);
+              if (!UNIFORM) {
+                s0 = mul2(s0, ls);
+                s1 = mul2(s1, ls);
+              }
+              f32x2 &v0 = v[(c * STEP + j) / 2], &v1 = v[(c * STEP + j) / 2 + 1];
+              v0 = fma2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), s0, v0);
+              v1 = fma2(pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), s1, v1);
+            }
+          }
+        }
+      }
+      if (n >= o.n) continue;
+      const float poison = sums.ok ? 0.0f : __uint_as_float(0x7fc00000u);
+      T *col = p.out + m0 * o.out_stride + n;
+      const int rows = m0 < o.m ? (int)min((uint64_t)COLS, o.m - m0) : 0;
+#pragma unroll
+      for (int j = 0; j < COLS / 2; j++) {
+        float x, y;
+        unpack2(v[j], x, y);
+        if (2 * j < rows) col[(uint64_t)(2 * j) * o.out_stride] = from_float<T>(x + poison);
+        if (2 * j + 1 < rows) col[(uint64_t)(2 * j + 1) * o.out_stride] = from_float<T>(y + poison);
+      }
+    }
+  }
+};
+
+template <int COLS, bool UNIFORM, typename T>
+cudaError_t launch_tiles(const Operands &o, T *out, int sms, cudaStream_t st) {
+  using Op = BlocksOp<COLS, UNIFORM, T>;
+  typename Op::Args args = {};
+  args.bn = 2 * COLS;
+  args.mt = (uint32_t)((o.m + 2 * COLS - 1) / (2 * COLS));
+  args.nt = (uint32_t)((o.n + 255) / 256);
+  args.o = o;
+  args.out = out;
+  if (!encode_operand_map(args.a, 1, o.b, o.k, o.n, o.b_stride, 128) ||
+      !encode_operand_map(args.b, 1, o.a, o.k, o.m, o.a_stride, COLS))
+    return cudaErrorInvalidValue;
+  return launch_pair<Op>(args, args.mt * args.nt, sms, st);
+}
+
+template <typename T>
+cudaError_t launch_matmul(const Operands &o, T *out, cudaStream_t st) {
+  if (o.m <= 4) {
+    const unsigned grid = (unsigned)((o.n + 8 * kFewRows - 1) / (8 * kFewRows));
+    if (o.m == 1) matmul_few<1><<<grid, 256, 0, st>>>(o, out);
+    else if (o.m == 2) matmul_few<2><<<grid, 256, 0, st>>>(o, out);
+    else matmul_few<4><<<grid, 256, 0, st>>>(o, out);
+    return cudaGetLastError();
+  }
+  const int sms = op_sms();
+  if (sms < 2) return cudaErrorNoDevice;
+  const bool uniform = o.b_shift != 0;
+  // columns a thread: the fewest that hold a's rows in one tile
+  if (o.m <= 32) return uniform ? launch_tiles<16, true>(o, out, sms, st) : launch_tiles<16, false>(o, out, sms, st);
+  if (o.m <= 128) return uniform ? launch_tiles<64, true>(o, out, sms, st) : launch_tiles<64, false>(o, out, sms, st);
+  return uniform ? launch_tiles<128, true>(o, out, sms, st) : launch_tiles<128, false>(o, out, sms, st);
 }
 
 }  // namespace
@@ -103,22 +409,18 @@ extern "C" int AnnB200QuantizeBlocks(uint32_t dtype, const void *x, uint64_t str
   if (!x || !codes || !scales) return report_error(OP_INVALID, "NULL pointer");
   if (stride < k || code_stride < k || code_stride % 16 || reinterpret_cast<uintptr_t>(codes) % 16)
     return report_error(OP_INVALID, "rows overlap, or code rows are not 16-byte aligned");
+  if (m * ((k + kBlock - 1) / kBlock) > 0x7fffffffull * 64)
+    return report_error(OP_INVALID, "more than 2^37 blocks");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const uint32_t kb = (k + kBlock - 1) / kBlock, height = square ? kBlock : 1;
-  const uint64_t blocks = (m + height - 1) / height * kb;
-  if (blocks > 0x7fffffffull) return report_error(OP_INVALID, "more than 2^31 blocks");
   switch (dtype) {
     case ANNB200_F32:
-      quantize<<<(unsigned)blocks, 128, 0, st>>>(static_cast<const float *>(x), stride, m, k, height, codes,
-                                                 code_stride, scales);
+      launch_quantize(static_cast<const float *>(x), stride, m, k, square != 0, codes, code_stride, scales, st);
       break;
     case ANNB200_F16:
-      quantize<<<(unsigned)blocks, 128, 0, st>>>(static_cast<const __half *>(x), stride, m, k, height, codes,
-                                                 code_stride, scales);
+      launch_quantize(static_cast<const __half *>(x), stride, m, k, square != 0, codes, code_stride, scales, st);
       break;
     default:
-      quantize<<<(unsigned)blocks, 128, 0, st>>>(static_cast<const __nv_bfloat16 *>(x), stride, m, k, height, codes,
-                                                 code_stride, scales);
+      launch_quantize(static_cast<const __nv_bfloat16 *>(x), stride, m, k, square != 0, codes, code_stride, scales, st);
   }
   return op_launched("quantize blocks", 1);
 }
@@ -141,30 +443,14 @@ extern "C" int AnnB200MatmulBlocks(const uint8_t *a, uint64_t a_stride, const fl
   if (a_stride < k || b_stride < k || a_stride % 16 || b_stride % 16 || reinterpret_cast<uintptr_t>(a) % 16 ||
       reinterpret_cast<uintptr_t>(b) % 16)
     return report_error(OP_INVALID, "rows of codes overlap, or are not 16-byte aligned");
-  const uint32_t sa = a_square ? 7 : 0, sb = b_square ? 7 : 0;
-  // the grid's y dimension takes 65,535 tiles: more rows go in several launches
-  const uint64_t rows = 65535ull * 64;
-  unsigned long long launches = 0;
-  for (uint64_t r = 0; r < m; r += rows) {
-    const uint64_t mm = std::min(rows, m - r);
-    const dim3 grid((unsigned)((n + 63) / 64), (unsigned)((mm + 63) / 64));
-    const uint8_t *ar = a + r * a_stride;
-    const float *as = a_scales + (r >> sa) * ((k + kBlock - 1) / kBlock);
-    const uint64_t o = r * out_stride;
-    switch (out_dtype) {
-      case ANNB200_F32:
-        matmul<<<grid, 256, 0, st>>>(ar, a_stride, as, sa, b, b_stride, b_scales, sb, mm, n, k,
-                                     static_cast<float *>(out) + o, out_stride);
-        break;
-      case ANNB200_F16:
-        matmul<<<grid, 256, 0, st>>>(ar, a_stride, as, sa, b, b_stride, b_scales, sb, mm, n, k,
-                                     static_cast<__half *>(out) + o, out_stride);
-        break;
-      default:
-        matmul<<<grid, 256, 0, st>>>(ar, a_stride, as, sa, b, b_stride, b_scales, sb, mm, n, k,
-                                     static_cast<__nv_bfloat16 *>(out) + o, out_stride);
-    }
-    launches++;
+  const Operands o = {a, b, a_stride, b_stride, a_scales, b_scales, a_square ? 7u : 0u, b_square ? 7u : 0u, m, n, k,
+                      (k + kBlock - 1) / kBlock, out_stride};
+  cudaError_t e;
+  switch (out_dtype) {
+    case ANNB200_F32: e = launch_matmul(o, static_cast<float *>(out), st); break;
+    case ANNB200_F16: e = launch_matmul(o, static_cast<__half *>(out), st); break;
+    default: e = launch_matmul(o, static_cast<__nv_bfloat16 *>(out), st);
   }
-  return op_launched("matmul blocks", launches);
+  if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "matmul blocks: %s", cudaGetErrorString(e));
+  return op_launched("matmul blocks", 1);
 }

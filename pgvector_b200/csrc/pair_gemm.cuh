@@ -29,6 +29,8 @@
 // epilogue goes through its remaining items with NaN for their sums.
 #pragma once
 
+#include <atomic>
+
 #include "ops.cuh"
 #include "tc.cuh"
 
@@ -431,8 +433,17 @@ template <class Op>
 cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, cudaStream_t st) {
   const int b_bytes = (int)args.bn * 64;
   const int smem = PairShape<Op>::smem(b_bytes);
-  cudaError_t e = cudaFuncSetAttribute(pair_gemm<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // the attribute is a device's: set once on each
+  static std::atomic<uint64_t> set{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(set.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(pair_gemm<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+    if (e != cudaSuccess) return e;
+    set.fetch_or(bit, std::memory_order_relaxed);
+  }
   const uint32_t clusters = items < (uint32_t)(sms / 2) ? items : (uint32_t)(sms / 2);
   pair_gemm<Op><<<2 * clusters, kPairThreads, smem, st>>>(args);
   return cudaGetLastError();
