@@ -252,15 +252,22 @@ __global__ void __launch_bounds__(256, M == 1 ? 3 : 2) matmul_few(const Operands
 // ---------------------------------------------------------------- product, tensor cores
 
 // Tiles of 256 of b's rows (lanes) x 2 COLS of a's (columns, COLS a thread).
-// UNIFORM: b's scales are square, so a warp's rows share them and they join
-// a's in shared memory: one multiply-add a value instead of two operations.
+// Two helper warps bring the scales, of which a K block needs one a row and a
+// column: AHEAD blocks at a time (16 bytes of a scale row) into one of two
+// buffers, laid out so that the epilogue reads four columns' at once.
+// UNIFORM: b's scales are square, so a CTA's 128 rows share them and the
+// helpers multiply them into a's: one multiply-add a value instead of two
+// operations. The epilogue's 128 sums a thread leave it few registers: all
+// else of a block comes from shared memory.
 template <int COLS, bool UNIFORM, typename T>
 struct BlocksOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1;
-  static constexpr int AHEAD = 4;   // blocks whose scales are staged at a time
-  static constexpr int SCRATCH = 2 * AHEAD * 2 * COLS * 4;
+  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  static constexpr int AHEAD = 4;
+  static constexpr int ROW = 2 * COLS + (UNIFORM ? 0 : 128);   // scales of a block: columns', then rows'
+  static constexpr int BUFFER = AHEAD * ROW * 4;
+  static constexpr int SCRATCH = 2 * BUFFER + 64;
   struct Args {
     CUtensorMap a[1], b[1];   // the tile's rows (the product's b) and columns (its a)
     uint32_t bn;              // 2 COLS
@@ -271,6 +278,15 @@ struct BlocksOp {
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
     return {(int32_t)((i / p.mt) * 256), (int32_t)((i % p.mt) * p.bn), 0, p.o.kb, 0};
+  }
+  static __device__ __forceinline__ uint64_t *bars(uint8_t *scratch) {   // full[2], empty[2]
+    return reinterpret_cast<uint64_t *>(scratch + 2 * BUFFER);
+  }
+  static __device__ __forceinline__ void init(uint8_t *scratch) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(bars(scratch) + i, HELPERS);
+      mbar_init(bars(scratch) + 2 + i, kPairEpiWarps);
+    }
   }
   // Scales b0 .. b0 + 3 of a row of blocks (0 past the last).
   static __device__ __forceinline__ float4 scales4(const float *row, uint32_t b0, uint32_t kb) {
@@ -283,70 +299,119 @@ struct BlocksOp {
     v.w = b0 + 3 < kb ? __ldg(row + b0 + 3) : 0.0f;
     return v;
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
-                                                  uint32_t cluster, uint32_t clusters) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
-    float *stage = reinterpret_cast<float *>(scratch) + half * COLS;   // [2][AHEAD][2 COLS]
+  static __device__ __forceinline__ void help(const Args &p, uint8_t *scratch, uint32_t rank, uint32_t cluster,
+                                              uint32_t clusters, volatile uint32_t *abort) {
     const Operands &o = p.o;
+    const uint32_t t = threadIdx.x - 320, lane = threadIdx.x & 31;
+    constexpr int EACH = (ROW + 63) / 64;
     uint32_t group = 0;
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
-      const uint64_t n = (uint64_t)w.a_row + rank * 128 + quad * 32 + lane;   // b's row
-      const uint64_t m0 = (uint64_t)w.b_row + half * COLS;                    // a's first row
-      const float *lane_scales = o.b_scales + (min(n, o.n - 1) >> o.b_shift) * o.kb;
-      // the half's four warps stage COLS rows' scales between them
-      const uint32_t mine = quad * 32 + lane;
-      const bool stages = mine < COLS;
-      const float *col_scales = o.a_scales + (min(m0 + mine, o.m - 1) >> o.a_shift) * o.kb;
+      const uint64_t n0 = (uint64_t)w.a_row + rank * 128, m0 = (uint64_t)w.b_row;
+      const float *row[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; e++) {
+        const uint32_t c = t + 64 * e;
+        row[e] = c < 2 * COLS ? o.a_scales + (min(m0 + c, o.m - 1) >> o.a_shift) * o.kb
+                              : o.b_scales + (min(n0 + c - 2 * COLS, o.n - 1) >> o.b_shift) * o.kb;
+      }
+      const float *shared_row = o.b_scales + (min(n0, o.n - 1) >> o.b_shift) * o.kb;
+      for (uint32_t b0 = 0; b0 < o.kb; b0 += AHEAD, group++) {
+        float4 v[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) v[e] = scales4(row[e], b0, o.kb);
+        if (UNIFORM) {
+          const float4 s = scales4(shared_row, b0, o.kb);
+#pragma unroll
+          for (int e = 0; e < EACH; e++) v[e] = make_float4(v[e].x * s.x, v[e].y * s.y, v[e].z * s.z, v[e].w * s.w);
+        }
+        uint64_t *bar = bars(scratch) + (group & 1);
+        if (!pair_wait(bar + 2, ((group >> 1) & 1) ^ 1, abort)) return;
+        float *at = reinterpret_cast<float *>(scratch + (group & 1) * BUFFER);
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+          const uint32_t c = t + 64 * e;
+          if (c < ROW) {
+            at[c] = v[e].x;
+            at[ROW + c] = v[e].y;
+            at[2 * ROW + c] = v[e].z;
+            at[3 * ROW + c] = v[e].w;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      }
+    }
+  }
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+                                                  uint32_t cluster, uint32_t clusters) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
+    uint32_t group = 0;
+    for (uint32_t i = cluster; i < items(p); i += clusters) {
       f32x2 v[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; j++) v[j] = 0;
-      float4 sb = scales4(lane_scales, 0, o.kb), sa = stages ? scales4(col_scales, 0, o.kb) : make_float4(0, 0, 0, 0);
-      for (uint32_t b0 = 0; b0 < o.kb; b0 += AHEAD, group++) {
-        float *at = stage + (group & 1) * (AHEAD * 2 * COLS);
-        const float4 own = sb;
-        if (stages) {
-          at[mine] = UNIFORM ? sa.x * own.x : sa.x;
-          at[2 * COLS + mine] = UNIFORM ? sa.y * own.y : sa.y;
-          at[4 * COLS + mine] = UNIFORM ? sa.z * own.z : sa.z;
-          at[6 * COLS + mine] = UNIFORM ? sa.w * own.w : sa.w;
-        }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-        if (b0 + AHEAD < o.kb) {   // the next group's, under this one's products
-          sb = scales4(lane_scales, b0 + AHEAD, o.kb);
-          if (stages) sa = scales4(col_scales, b0 + AHEAD, o.kb);
-        }
 #pragma unroll 1
-        for (uint32_t g = 0; g < AHEAD && b0 + g < o.kb; g++) {
-          const uint32_t addr = sums.acquire() + half * COLS;
-          const float *scale = at + g * 2 * COLS;
-          const float l = g == 0 ? own.x : (g == 1 ? own.y : (g == 2 ? own.z : own.w));
-          const f32x2 ls = pack2(l, l);
-          constexpr int STEP = COLS < 32 ? COLS : 32;
+      for (uint32_t b = 0; b < p.o.kb; b++) {
+        const uint32_t g = b % AHEAD;
+        uint64_t *bar = bars(scratch) + (group & 1);
+        if (g == 0 && sums.ok) sums.ok = __all_sync(0xffffffffu, pair_wait(bar, (group >> 1) & 1, sums.abort));
+        uint32_t scale = smem_u32(scratch) + (group & 1) * BUFFER + g * ROW * 4;
+        const uint32_t addr = sums.acquire() + half * COLS;
+        f32x2 ls = 0;
+        if (!UNIFORM) {
+          float l;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(l) : "r"(scale + (2 * COLS + quad * 32 + lane) * 4));
+          ls = pack2(l, l);
+        }
+        scale += half * COLS * 4;
+        if (sums.ok) {
+          // COLS columns in steps, one read of tensor memory ahead
+          constexpr int STEP = COLS < 32 ? COLS : 32, STEPS = COLS / STEP;
+          uint32_t r[2][STEP];
+          auto read = [&](int c, uint32_t(&to)[STEP]) {
+            if constexpr (STEP == 32) TMEM_LD32(addr + c * 32, to);
+            else TMEM_LD16(addr, to);
+          };
+          auto wait = [&](uint32_t(&to)[STEP]) {
+            tmem_ld_wait();
+            if constexpr (STEP == 32) TMEM_KEEP32(to);
+            else TMEM_KEEP16(to);
+          };
+          read(0, r[0]);
+          wait(r[0]);
 #pragma unroll
-          for (int c = 0; c < COLS / STEP; c++) {
-            uint32_t r[STEP];
-            if (sums.ok) {
-              if constexpr (STEP == 32) TMEM_LD32(addr + c * 32, r);
-              else TMEM_LD16(addr, r);
-              tmem_ld_wait();
-            }
-            if (c + 1 == COLS / STEP) sums.release();
+          for (int c = 0; c < STEPS; c++) {
+            if (c + 1 < STEPS) read(c + 1, r[(c + 1) & 1]);
 #pragma unroll
             for (int j = 0; j < STEP; j += 4) {
-              const float4 s4 = *reinterpret_cast<const float4 *>(scale + c * STEP + j);
-              f32x2 s0 = pack2(s4.x, s4.y), s1 = pack2(s4.z, s4.w);
+              const uint32_t(&q)[STEP] = r[c & 1];
+              // (volatile: in order with the reads of tensor memory, not all ahead of them in registers)
+              f32x2 s0, s1;
+              asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
+                           : "=l"(s0), "=l"(s1)
+                           : "r"(scale + (c * STEP + j) * 4));
               if (!UNIFORM) {
                 s0 = mul2(s0, ls);
                 s1 = mul2(s1, ls);
               }
               f32x2 &v0 = v[(c * STEP + j) / 2], &v1 = v[(c * STEP + j) / 2 + 1];
-              v0 = fma2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), s0, v0);
-              v1 = fma2(pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), s1, v1);
+              v0 = fma2(pack2(__uint_as_float(q[j]), __uint_as_float(q[j + 1])), s0, v0);
+              v1 = fma2(pack2(__uint_as_float(q[j + 2]), __uint_as_float(q[j + 3])), s1, v1);
             }
+            if (c + 1 < STEPS) wait(r[(c + 1) & 1]);
           }
         }
+        sums.release();
+        if (g + 1 == AHEAD || b + 1 == p.o.kb) {
+          if (lane == 0) mbar_arrive(bar + 2);
+          group++;
+        }
       }
+      const PairItem w = item(p, i);
+      const Operands &o = p.o;
+      const uint64_t n = (uint64_t)w.a_row + rank * 128 + quad * 32 + lane;   // b's row
+      const uint64_t m0 = (uint64_t)w.b_row + half * COLS;                    // a's first row
       if (n >= o.n) continue;
       const float poison = sums.ok ? 0.0f : __uint_as_float(0x7fc00000u);
       T *col = p.out + m0 * o.out_stride + n;
@@ -355,8 +420,10 @@ struct BlocksOp {
       for (int j = 0; j < COLS / 2; j++) {
         float x, y;
         unpack2(v[j], x, y);
-        if (2 * j < rows) col[(uint64_t)(2 * j) * o.out_stride] = from_float<T>(x + poison);
-        if (2 * j + 1 < rows) col[(uint64_t)(2 * j + 1) * o.out_stride] = from_float<T>(y + poison);
+        if (2 * j < rows) *col = from_float<T>(x + poison);
+        col += o.out_stride;
+        if (2 * j + 1 < rows) *col = from_float<T>(y + poison);
+        col += o.out_stride;
       }
     }
   }

@@ -175,7 +175,7 @@ template <> __device__ __forceinline__ uint32_t round2<__half>(f32x2 v, f32x2 &k
 
 // Tiles of 256 queries x 256 rows. GRAD: G of a piece; else the partial sums.
 template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
-struct LogitsOp {
+struct LogitsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? kPairEpiWarps * kBoxBytes : 0, MAX_STAGES = 8;
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(128) join_parts(const float2 *part, uint32_t n
 
 // dX partial sums: 256 queries x bn dimensions, K = a share of the piece's rows.
 template <PairKind KIND_, int PLANES_>
-struct QueriesOp {
+struct QueriesOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = true;
   static constexpr int PLANES = PLANES_, SCRATCH = kPairEpiWarps * kBoxBytes, MAX_STAGES = 8;
@@ -467,7 +467,7 @@ struct QueriesOp {
 
 // dW: 256 of the piece's rows x bn dimensions, K = the queries.
 template <PairKind KIND_, int PLANES_, typename T>
-struct RowsOp {
+struct RowsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = true, B_MN = true;
   static constexpr int PLANES = PLANES_, SCRATCH = kPairEpiWarps * kBoxBytes, MAX_STAGES = 8;

@@ -14,6 +14,7 @@
 //              completing on the leader CTA's barrier.
 //   warp 9     MMA issuer (leader CTA); tcgen05.commit frees the stage and
 //              publishes the sums in both CTAs.
+//   warps 10, 11  an operator's helpers, if it has any.
 //
 // Two sums of 256 columns each let the epilogue of one run under the products
 // of the next. The tensor cores cut off, and do not round, what falls below a
@@ -37,7 +38,12 @@
 namespace annb200 {
 
 constexpr int kPairEpiWarps = 8;
-constexpr int kPairThreads = 32 * (kPairEpiWarps + 2);
+constexpr int kPairThreads = 32 * (kPairEpiWarps + 4);   // three warpgroups, for the register split
+// Registers a thread: 384 threads start with 168 each. The epilogue's 256 go up
+// to 224 and the other 128 down to 56: 256 * 224 + 128 * 56 = 384 * 168. Each
+// side asks for its share at the top of its own branch, which no other joins.
+constexpr int kPairEpiRegs = 224, kPairOtherRegs = 56;
+static_assert(256 * kPairEpiRegs + 128 * kPairOtherRegs <= 384 * 168, "more registers than the block starts with");
 constexpr int kPairTileBytes = 128 * 128;     // 128 rows of 128 bytes (or 128 bytes wide, 128 K rows)
 constexpr int kPairSmem = 227 * 1024;
 
@@ -212,14 +218,22 @@ struct PairSums {
     for (uint32_t kb = 0; kb < kblocks; kb += CHUNK) {
       const uint32_t addr = acquire() + at;
       if (ok) {
+        // one read ahead of the additions
+        uint32_t r[2][32];
+        TMEM_LD32(addr, r[0]);
+        tmem_ld_wait();
+        TMEM_KEEP32(r[0]);
 #pragma unroll
         for (int c = 0; c < N; c++) {
-          uint32_t r[32];
-          TMEM_LD32(addr + c * 32, r);
-          tmem_ld_wait();
+          if (c + 1 < N) TMEM_LD32(addr + (c + 1) * 32, r[(c + 1) & 1]);
 #pragma unroll
           for (int j = 0; j < 16; j++)
-            v[16 * c + j] = add2(v[16 * c + j], pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+            v[16 * c + j] = add2(v[16 * c + j],
+                                 pack2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])));
+          if (c + 1 < N) {
+            tmem_ld_wait();
+            TMEM_KEEP32(r[(c + 1) & 1]);
+          }
         }
       }
       release();
@@ -234,6 +248,7 @@ struct PairSums {
     if (ok) {
       TMEM_LD32(addr, r);
       tmem_ld_wait();
+      TMEM_KEEP32(r);
     } else {
 #pragma unroll
       for (int j = 0; j < 32; j++) r[j] = 0x7fc00000u;
@@ -257,9 +272,18 @@ struct PairShape {
 };
 
 // Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
-// sum; 0: the item's), Args with maps a[PLANES],
+// sum; 0: the item's), HELPERS (0 or 2 warps), Args with maps a[PLANES],
 // b[PLANES] and bn (columns of a tile), items(args), item(args, i),
-// epilogue(args, sums, scratch, rank, cluster, clusters): all of the cluster's items.
+// epilogue(args, sums, scratch, rank, cluster, clusters): all of the cluster's
+// items; init and help where there are helpers.
+struct PairNoHelpers {
+  static constexpr int HELPERS = 0;
+  static __device__ __forceinline__ void init(uint8_t *) {}
+  template <class Args>
+  static __device__ __forceinline__ void help(const Args &, uint8_t *, uint32_t, uint32_t, uint32_t,
+                                              volatile uint32_t *) {}
+};
+
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_gemm(const __grid_constant__ typename Op::Args args) {
@@ -287,6 +311,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t items = Op::items(args);
 
   if (threadIdx.x == 0) {
+    Op::init(scratch);
     for (uint32_t s = 0; s < stages; s++) {
       mbar_init(full + s, 1);
       mbar_init(empty + s, 1);
@@ -311,113 +336,119 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 8) {
-    if (lane == 0) {
-      uint32_t s = 0, round = 0;
-      bool ok = true;
-      for (uint32_t i = cluster; i < items && ok; i += clusters) {
-        const PairItem w = Op::item(args, i);
-        const int32_t ar = w.a_row + (int32_t)rank * 128, br = w.b_row + (int32_t)(rank * (args.bn / 2));
-        for (uint32_t kb = 0; kb < w.kblocks; kb++) {
-          if (!pair_wait(empty + s, (round & 1) ^ 1, abort)) {
-            ok = false;
-            break;
-          }
-          const uint32_t bar = map_to_leader(smem_u32(full + s));
-          if (rank == 0) mbar_expect_tx(full + s, 2 * stage_bytes);
-          const int32_t k = w.k0 + (int32_t)(kb * KE);
-          const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
-#pragma unroll
-          for (int p = 0; p < PLANES; p++) {
-            if (Op::A_MN) {
-              pair_load(a + p * kPairTileBytes, &args.a[p], ar, k, bar);
-              pair_load(a + p * kPairTileBytes + 8192, &args.a[p], ar + 64, k, bar);
-            } else {
-              pair_load(a + p * kPairTileBytes, &args.a[p], k, ar, bar);
-            }
-            if (Op::B_MN) {
-              for (uint32_t c = 0; c < args.bn / 2; c += 64)
-                pair_load(b + p * b_bytes + c * 128, &args.b[p], br + (int32_t)c, k, bar);
-            } else {
-              pair_load(b + p * b_bytes, &args.b[p], k, br, bar);
-            }
-          }
-          if (++s == stages) {
-            s = 0;
-            round++;
-          }
-        }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = pair_idesc<Op::KIND, Op::A_MN, Op::B_MN>(args.bn);
-      constexpr uint32_t A_STEP = Op::A_MN ? 2048 : 32, B_STEP = Op::B_MN ? 2048 : 32;
-      uint32_t s = 0, round = 0, acc = 0;
-      bool ok = true;
-      for (uint32_t i = cluster; i < items && ok; i += clusters) {
-        const PairItem w = Op::item(args, i);
-        for (uint32_t kb = 0; kb < w.kblocks; kb++) {
-          const bool first = Op::CHUNK ? kb % (Op::CHUNK + !Op::CHUNK) == 0 : kb == 0;
-          const bool last = kb + 1 == w.kblocks || (Op::CHUNK && (kb + 1) % (Op::CHUNK + !Op::CHUNK) == 0);
-          if (first && !pair_wait(tempty + (acc & 1), ((acc >> 1) & 1) ^ 1, abort)) {
-            ok = false;
-            break;
-          }
-          if (!pair_wait(full + s, round & 1, abort)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t d = tmem + (acc & 1) * 256;
-          const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
-          auto adesc = [&](uint32_t p, uint32_t kk) {
-            const uint32_t at = a + p * kPairTileBytes + kk * A_STEP;
-            return Op::A_MN ? sw128_mn_desc(at, 8192) : sw128_desc(at);
-          };
-          auto bdesc = [&](uint32_t p, uint32_t kk) {
-            const uint32_t at = b + p * b_bytes + kk * B_STEP;
-            return Op::B_MN ? sw128_mn_desc(at, 8192) : sw128_desc(at);
-          };
-#pragma unroll
-          for (uint32_t kk = 0; kk < 4; kk++) {
-            pair_mma<Op::KIND>(d, adesc(0, kk), bdesc(0, kk), idesc, !(first && kk == 0));
-            if (PLANES == 2) {   // high by low and low by high terms; low by low is below FP32's half step
-              pair_mma<Op::KIND>(d, adesc(0, kk), bdesc(1, kk), idesc, 1u);
-              pair_mma<Op::KIND>(d, adesc(1, kk), bdesc(0, kk), idesc, 1u);
-            }
-          }
-          pair_commit(empty + s);
-          if (last) {
-            pair_commit(tfull + (acc & 1));
-            acc++;
-          }
-          if (++s == stages) {
-            s = 0;
-            round++;
-          }
-        }
-      }
-      // the MMAs issued have ended, and the loads in flight have landed, before anything is freed
-      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain))
-                   : "memory");
-      uint64_t t0 = globaltimer();
-      while (!mbar_try_wait(drain, 0) && globaltimer() - t0 < kWaitNs) {
-      }
-      if (*abort) {
-        t0 = globaltimer();
-        for (uint32_t s = 0; s < stages; s++)
-          for (uint32_t parity = 0; parity < 2; parity++)
-            while (!mbar_try_wait(full + s, parity) && globaltimer() - t0 < kWaitNs) {
-            }
-      }
-    }
-    __syncwarp();
-  } else {
+  if (warp < kPairEpiWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpiRegs));
     PairSums sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
     Op::epilogue(args, sums, scratch, rank, cluster, clusters);
     BoxStore::finish();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairOtherRegs));
+    if (warp == 8) {
+      if (lane == 0) {
+        uint32_t s = 0, round = 0;
+        bool ok = true;
+        for (uint32_t i = cluster; i < items && ok; i += clusters) {
+          const PairItem w = Op::item(args, i);
+          const int32_t ar = w.a_row + (int32_t)rank * 128, br = w.b_row + (int32_t)(rank * (args.bn / 2));
+          for (uint32_t kb = 0; kb < w.kblocks; kb++) {
+            if (!pair_wait(empty + s, (round & 1) ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bar = map_to_leader(smem_u32(full + s));
+            if (rank == 0) mbar_expect_tx(full + s, 2 * stage_bytes);
+            const int32_t k = w.k0 + (int32_t)(kb * KE);
+            const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
+#pragma unroll
+            for (int p = 0; p < PLANES; p++) {
+              if (Op::A_MN) {
+                pair_load(a + p * kPairTileBytes, &args.a[p], ar, k, bar);
+                pair_load(a + p * kPairTileBytes + 8192, &args.a[p], ar + 64, k, bar);
+              } else {
+                pair_load(a + p * kPairTileBytes, &args.a[p], k, ar, bar);
+              }
+              if (Op::B_MN) {
+                for (uint32_t c = 0; c < args.bn / 2; c += 64)
+                  pair_load(b + p * b_bytes + c * 128, &args.b[p], br + (int32_t)c, k, bar);
+              } else {
+                pair_load(b + p * b_bytes, &args.b[p], k, br, bar);
+              }
+            }
+            if (++s == stages) {
+              s = 0;
+              round++;
+            }
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      if (lane == 0 && rank == 0) {
+        const uint32_t idesc = pair_idesc<Op::KIND, Op::A_MN, Op::B_MN>(args.bn);
+        constexpr uint32_t A_STEP = Op::A_MN ? 2048 : 32, B_STEP = Op::B_MN ? 2048 : 32;
+        uint32_t s = 0, round = 0, acc = 0;
+        bool ok = true;
+        for (uint32_t i = cluster; i < items && ok; i += clusters) {
+          const PairItem w = Op::item(args, i);
+          for (uint32_t kb = 0; kb < w.kblocks; kb++) {
+            const bool first = Op::CHUNK ? kb % (Op::CHUNK + !Op::CHUNK) == 0 : kb == 0;
+            const bool last = kb + 1 == w.kblocks || (Op::CHUNK && (kb + 1) % (Op::CHUNK + !Op::CHUNK) == 0);
+            if (first && !pair_wait(tempty + (acc & 1), ((acc >> 1) & 1) ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            if (!pair_wait(full + s, round & 1, abort)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d = tmem + (acc & 1) * 256;
+            const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
+            auto adesc = [&](uint32_t p, uint32_t kk) {
+              const uint32_t at = a + p * kPairTileBytes + kk * A_STEP;
+              return Op::A_MN ? sw128_mn_desc(at, 8192) : sw128_desc(at);
+            };
+            auto bdesc = [&](uint32_t p, uint32_t kk) {
+              const uint32_t at = b + p * b_bytes + kk * B_STEP;
+              return Op::B_MN ? sw128_mn_desc(at, 8192) : sw128_desc(at);
+            };
+#pragma unroll
+            for (uint32_t kk = 0; kk < 4; kk++) {
+              pair_mma<Op::KIND>(d, adesc(0, kk), bdesc(0, kk), idesc, !(first && kk == 0));
+              if (PLANES == 2) {   // high by low and low by high terms; low by low is below FP32's half step
+                pair_mma<Op::KIND>(d, adesc(0, kk), bdesc(1, kk), idesc, 1u);
+                pair_mma<Op::KIND>(d, adesc(1, kk), bdesc(0, kk), idesc, 1u);
+              }
+            }
+            pair_commit(empty + s);
+            if (last) {
+              pair_commit(tfull + (acc & 1));
+              acc++;
+            }
+            if (++s == stages) {
+              s = 0;
+              round++;
+            }
+          }
+        }
+        // the MMAs issued have ended, and the loads in flight have landed, before anything is freed
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain))
+                     : "memory");
+        uint64_t t0 = globaltimer();
+        while (!mbar_try_wait(drain, 0) && globaltimer() - t0 < kWaitNs) {
+        }
+        if (*abort) {
+          t0 = globaltimer();
+          for (uint32_t s = 0; s < stages; s++)
+            for (uint32_t parity = 0; parity < 2; parity++)
+              while (!mbar_try_wait(full + s, parity) && globaltimer() - t0 < kWaitNs) {
+              }
+        }
+      }
+      __syncwarp();
+    } else if (Op::HELPERS) {
+      Op::help(args, scratch, rank, cluster, clusters, abort);
+    }
   }
   tc_fence_before();
   __syncthreads();
