@@ -348,9 +348,9 @@ struct BlocksOp {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
     uint32_t group = 0;
     for (uint32_t i = cluster; i < items(p); i += clusters) {
-      f32x2 v[COLS / 2];
+      float v[COLS];
 #pragma unroll
-      for (int j = 0; j < COLS / 2; j++) v[j] = 0;
+      for (int j = 0; j < COLS; j++) v[j] = 0.0f;
 #pragma unroll 1
       for (uint32_t b = 0; b < p.o.kb; b++) {
         const uint32_t g = b % AHEAD;
@@ -395,9 +395,15 @@ struct BlocksOp {
                 s0 = mul2(s0, ls);
                 s1 = mul2(s1, ls);
               }
-              f32x2 &v0 = v[(c * STEP + j) / 2], &v1 = v[(c * STEP + j) / 2 + 1];
-              v0 = fma2(pack2(__uint_as_float(q[j]), __uint_as_float(q[j + 1])), s0, v0);
-              v1 = fma2(pack2(__uint_as_float(q[j + 2]), __uint_as_float(q[j + 3])), s1, v1);
+              // (one value at a time: pairing what tensor memory gives costs more moves than it saves)
+              float t0, t1, t2, t3;
+              unpack2(s0, t0, t1);
+              unpack2(s1, t2, t3);
+              float *o = v + c * STEP + j;
+              o[0] = fmaf(__uint_as_float(q[j]), t0, o[0]);
+              o[1] = fmaf(__uint_as_float(q[j + 1]), t1, o[1]);
+              o[2] = fmaf(__uint_as_float(q[j + 2]), t2, o[2]);
+              o[3] = fmaf(__uint_as_float(q[j + 3]), t3, o[3]);
             }
             if (c + 1 < STEPS) wait(r[(c + 1) & 1]);
           }
@@ -417,12 +423,8 @@ struct BlocksOp {
       T *col = p.out + m0 * o.out_stride + n;
       const int rows = m0 < o.m ? (int)min((uint64_t)COLS, o.m - m0) : 0;
 #pragma unroll
-      for (int j = 0; j < COLS / 2; j++) {
-        float x, y;
-        unpack2(v[j], x, y);
-        if (2 * j < rows) *col = from_float<T>(x + poison);
-        col += o.out_stride;
-        if (2 * j + 1 < rows) *col = from_float<T>(y + poison);
+      for (int j = 0; j < COLS; j++) {
+        if (j < rows) *col = from_float<T>(v[j] + poison);
         col += o.out_stride;
       }
     }
