@@ -4,10 +4,9 @@
 //
 // The product has two kernels. With up to 4 rows in a (single queries) it is
 // bound by reading b once: a warp a few rows of b, CUDA cores. Above that the
-// tensor cores (pair_gemm.cuh), b's rows as the tile's 256 rows and a's as its
-// columns: a K block of 128 is one sum in tensor memory, which the epilogue
-// takes out, scales and adds up in FP32 registers while the next block's
-// products run.
+// tensor cores (pair_gemm.cuh): a K block of 128 is one sum in tensor memory,
+// which the epilogue takes out, scales and adds up in FP32 registers while the
+// next block's products run.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -251,171 +250,174 @@ __global__ void __launch_bounds__(256, M == 1 ? 3 : 2) matmul_few(const Operands
 
 // ---------------------------------------------------------------- product, tensor cores
 
-// Tiles of 256 of b's rows (lanes) x 2 COLS of a's (columns, COLS a thread).
-// Two helper warps bring the scales, of which a K block needs one a row and a
-// column: AHEAD blocks at a time (16 bytes of a scale row) into one of two
-// buffers, laid out so that the epilogue reads four columns' at once.
-// UNIFORM: b's scales are square, so a CTA's 128 rows share them and the
-// helpers multiply them into a's: one multiply-add a value instead of two
-// operations. The epilogue's 128 sums a thread leave it few registers: all
-// else of a block comes from shared memory.
-template <int COLS, bool UNIFORM, typename T>
-struct BlocksOp {
+// The scales of a K block, one a lane and one a column of the tile, for the
+// epilogues below: two helper warps bring AHEAD blocks at a time (16 bytes of
+// each scale row) into one of two buffers, transposed, so that lanes read
+// theirs side by side and columns' can be read several at once.
+//   LANES, COLS: scales a block (COLS 2: one for each half of the columns)
+template <int LANES_, int COLS_>
+struct ScaleStage {
+  static constexpr int LANES = LANES_, COLS = COLS_, ROW = LANES + (COLS < 4 ? 4 : COLS), AHEAD = 4;
+  static constexpr int BUFFER = AHEAD * ROW * 4;
+  static constexpr int BYTES = 2 * BUFFER + 64;
+  uint8_t *scratch;
+  uint32_t group = 0;
+  __device__ __forceinline__ uint64_t *bars() const { return reinterpret_cast<uint64_t *>(scratch + 2 * BUFFER); }
+  __device__ __forceinline__ void init() const {   // full[2], empty[2]
+    for (int i = 0; i < 2; i++) {
+      mbar_init(bars() + i, 2);
+      mbar_init(bars() + 2 + i, kPairEpiWarps);
+    }
+  }
+  // The helpers' part for one item: t = 0 .. 63; row(c): scale c's row of kb blocks.
+  template <typename Rows>
+  __device__ __forceinline__ bool fill(uint32_t t, const Rows &row_of, uint32_t kb, bool vec, volatile uint32_t *abort) {
+    constexpr int EACH = (LANES + COLS + 63) / 64;
+    const float *row[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) row[e] = row_of(min(t + 64 * e, (uint32_t)(LANES + COLS - 1)));
+    float4 v[EACH];
+    // blocks b0 .. b0 + 3 of each row (past the last: not used), all loads before any use
+    auto load = [&](uint32_t b0) {
+      if (vec) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) v[e] = __ldg(reinterpret_cast<const float4 *>(row[e] + b0));
+      } else {
+        const uint32_t last = kb - 1;
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+          v[e] = make_float4(__ldg(row[e] + b0), __ldg(row[e] + min(b0 + 1, last)), __ldg(row[e] + min(b0 + 2, last)),
+                             __ldg(row[e] + min(b0 + 3, last)));
+      }
+    };
+    load(0);
+    for (uint32_t b0 = 0; b0 < kb; b0 += AHEAD, group++) {
+      uint64_t *bar = bars() + (group & 1);
+      if (!pair_wait(bar + 2, ((group >> 1) & 1) ^ 1, abort)) return false;
+      float *at = reinterpret_cast<float *>(scratch + (group & 1) * BUFFER);
+#pragma unroll
+      for (int e = 0; e < EACH; e++) {
+        const uint32_t c = t + 64 * e;
+        if (c < LANES + COLS) {
+          at[c] = v[e].x;
+          at[ROW + c] = v[e].y;
+          at[2 * ROW + c] = v[e].z;
+          at[3 * ROW + c] = v[e].w;
+        }
+      }
+      __syncwarp();
+      if ((t & 31) == 0) mbar_arrive(bar);
+      if (b0 + AHEAD < kb) load(b0 + AHEAD);   // under the products of this group
+    }
+    return true;
+  }
+  // The epilogue's: shared address of block b's scales, and the end of its use.
+  __device__ __forceinline__ uint32_t take(uint32_t b, PairSums &sums) const {
+    if (b % AHEAD == 0 && sums.ok)
+      sums.ok = __all_sync(0xffffffffu, pair_wait(bars() + (group & 1), (group >> 1) & 1, sums.abort));
+    return smem_u32(scratch) + (group & 1) * BUFFER + (b % AHEAD) * (ROW * 4);
+  }
+  __device__ __forceinline__ void done(uint32_t b, uint32_t kb) {
+    if (b % AHEAD == AHEAD - 1 || b + 1 == kb) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(bars() + 2 + (group & 1));
+      group++;
+    }
+  }
+};
+__device__ __forceinline__ float shared_float(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+template <typename T>
+struct BlocksArgs {
+  CUtensorMap a[1], b[1];   // the tile's rows and columns
+  uint32_t bn;
+  uint32_t mt, nt;          // tiles of a's rows, of b's
+  Operands o;
+  T *out;
+  int boxes;                // out's rows are 16-byte aligned: `map` stores them
+  CUtensorMap map;
+};
+// Scales a and b both 16-byte aligned, and their rows: loads of four blocks.
+__device__ __forceinline__ bool scales_vec(const Operands &o) {
+  return (o.kb & 3) == 0 &&
+         ((reinterpret_cast<uintptr_t>(o.a_scales) | reinterpret_cast<uintptr_t>(o.b_scales)) & 15) == 0;
+}
+
+// Up to 128 rows in a: tiles of 256 of b's rows (lanes) x 2 COLS of a's (COLS a
+// thread), bound by reading b. A store of a column is 32 of b's rows side by side.
+template <int COLS, typename T>
+struct NarrowOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
-  static constexpr int AHEAD = 4;
-  static constexpr int ROW = 2 * COLS + (UNIFORM ? 0 : 128);   // scales of a block: columns', then rows'
-  static constexpr int BUFFER = AHEAD * ROW * 4;
-  static constexpr int SCRATCH = 2 * BUFFER + 64;
-  struct Args {
-    CUtensorMap a[1], b[1];   // the tile's rows (the product's b) and columns (its a)
-    uint32_t bn;              // 2 COLS
-    uint32_t mt, nt;          // tiles of a's rows, of b's
-    Operands o;
-    T *out;
-  };
+  using Scales = ScaleStage<128, 2 * COLS>;
+  static constexpr int SCRATCH = Scales::BYTES;
+  using Args = BlocksArgs<T>;
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
     return {(int32_t)((i / p.mt) * 256), (int32_t)((i % p.mt) * p.bn), 0, p.o.kb, 0};
   }
-  static __device__ __forceinline__ uint64_t *bars(uint8_t *scratch) {   // full[2], empty[2]
-    return reinterpret_cast<uint64_t *>(scratch + 2 * BUFFER);
-  }
-  static __device__ __forceinline__ void init(uint8_t *scratch) {
-    for (int i = 0; i < 2; i++) {
-      mbar_init(bars(scratch) + i, HELPERS);
-      mbar_init(bars(scratch) + 2 + i, kPairEpiWarps);
-    }
-  }
-  // Scales b0 .. b0 + 3 of a row of blocks (0 past the last).
-  static __device__ __forceinline__ float4 scales4(const float *row, uint32_t b0, uint32_t kb) {
-    if (b0 + 4 <= kb && (kb & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0)
-      return __ldg(reinterpret_cast<const float4 *>(row + b0));
-    float4 v;
-    v.x = b0 < kb ? __ldg(row + b0) : 0.0f;
-    v.y = b0 + 1 < kb ? __ldg(row + b0 + 1) : 0.0f;
-    v.z = b0 + 2 < kb ? __ldg(row + b0 + 2) : 0.0f;
-    v.w = b0 + 3 < kb ? __ldg(row + b0 + 3) : 0.0f;
-    return v;
-  }
+  static __device__ __forceinline__ void init(uint8_t *scratch) { Scales{scratch}.init(); }
   static __device__ __forceinline__ void help(const Args &p, uint8_t *scratch, uint32_t rank, uint32_t cluster,
                                               uint32_t clusters, volatile uint32_t *abort) {
     const Operands &o = p.o;
-    const uint32_t t = threadIdx.x - 320, lane = threadIdx.x & 31;
-    constexpr int EACH = (ROW + 63) / 64;
-    uint32_t group = 0;
+    Scales scales{scratch};
+    const bool vec = scales_vec(o);
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
       const uint64_t n0 = (uint64_t)w.a_row + rank * 128, m0 = (uint64_t)w.b_row;
-      const float *row[EACH];
-#pragma unroll
-      for (int e = 0; e < EACH; e++) {
-        const uint32_t c = t + 64 * e;
-        row[e] = c < 2 * COLS ? o.a_scales + (min(m0 + c, o.m - 1) >> o.a_shift) * o.kb
-                              : o.b_scales + (min(n0 + c - 2 * COLS, o.n - 1) >> o.b_shift) * o.kb;
-      }
-      const float *shared_row = o.b_scales + (min(n0, o.n - 1) >> o.b_shift) * o.kb;
-      for (uint32_t b0 = 0; b0 < o.kb; b0 += AHEAD, group++) {
-        float4 v[EACH];
-#pragma unroll
-        for (int e = 0; e < EACH; e++) v[e] = scales4(row[e], b0, o.kb);
-        if (UNIFORM) {
-          const float4 s = scales4(shared_row, b0, o.kb);
-#pragma unroll
-          for (int e = 0; e < EACH; e++) v[e] = make_float4(v[e].x * s.x, v[e].y * s.y, v[e].z * s.z, v[e].w * s.w);
-        }
-        uint64_t *bar = bars(scratch) + (group & 1);
-        if (!pair_wait(bar + 2, ((group >> 1) & 1) ^ 1, abort)) return;
-        float *at = reinterpret_cast<float *>(scratch + (group & 1) * BUFFER);
-#pragma unroll
-        for (int e = 0; e < EACH; e++) {
-          const uint32_t c = t + 64 * e;
-          if (c < ROW) {
-            at[c] = v[e].x;
-            at[ROW + c] = v[e].y;
-            at[2 * ROW + c] = v[e].z;
-            at[3 * ROW + c] = v[e].w;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-      }
+      if (!scales.fill(threadIdx.x - 320,
+                       [&](uint32_t c) {
+                         return c < 128 ? o.b_scales + (min(n0 + c, o.n - 1) >> o.b_shift) * o.kb
+                                        : o.a_scales + (min(m0 + c - 128, o.m - 1) >> o.a_shift) * o.kb;
+                       },
+                       o.kb, vec, abort))
+        return;
     }
   }
   static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
                                                   uint32_t cluster, uint32_t clusters) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
-    uint32_t group = 0;
+    const Operands &o = p.o;
+    Scales scales{scratch};
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       float v[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; j++) v[j] = 0.0f;
 #pragma unroll 1
-      for (uint32_t b = 0; b < p.o.kb; b++) {
-        const uint32_t g = b % AHEAD;
-        uint64_t *bar = bars(scratch) + (group & 1);
-        if (g == 0 && sums.ok) sums.ok = __all_sync(0xffffffffu, pair_wait(bar, (group >> 1) & 1, sums.abort));
-        uint32_t scale = smem_u32(scratch) + (group & 1) * BUFFER + g * ROW * 4;
-        const uint32_t addr = sums.acquire() + half * COLS;
-        f32x2 ls = 0;
-        if (!UNIFORM) {
-          float l;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(l) : "r"(scale + (2 * COLS + quad * 32 + lane) * 4));
-          ls = pack2(l, l);
-        }
-        scale += half * COLS * 4;
-        if (sums.ok) {
-          // COLS columns in steps, one read of tensor memory ahead
-          constexpr int STEP = COLS < 32 ? COLS : 32, STEPS = COLS / STEP;
-          uint32_t r[2][STEP];
-          auto read = [&](int c, uint32_t(&to)[STEP]) {
-            if constexpr (STEP == 32) TMEM_LD32(addr + c * 32, to);
-            else TMEM_LD16(addr, to);
-          };
-          auto wait = [&](uint32_t(&to)[STEP]) {
+      for (uint32_t b = 0; b < o.kb; b++) {
+        const uint32_t scale = scales.take(b, sums);
+        const uint32_t addr = sums.acquire() + half * COLS, cols = scale + (128 + half * COLS) * 4;
+        const float ls = shared_float(scale + (quad * 32 + lane) * 4);
+        constexpr int STEP = COLS < 32 ? COLS : 32;
+#pragma unroll
+        for (int c = 0; c < COLS; c += STEP) {
+          uint32_t r[STEP];
+          if (sums.ok) {
+            if constexpr (STEP == 32) TMEM_LD32(addr + c, r);
+            else TMEM_LD16(addr + c, r);
             tmem_ld_wait();
-            if constexpr (STEP == 32) TMEM_KEEP32(to);
-            else TMEM_KEEP16(to);
-          };
-          read(0, r[0]);
-          wait(r[0]);
+            if constexpr (STEP == 32) TMEM_KEEP32(r);
+            else TMEM_KEEP16(r);
+          }
 #pragma unroll
-          for (int c = 0; c < STEPS; c++) {
-            if (c + 1 < STEPS) read(c + 1, r[(c + 1) & 1]);
+          for (int j = 0; j < STEP; j += 4) {
+            float s[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(s[0]), "=f"(s[1]), "=f"(s[2]), "=f"(s[3])
+                         : "r"(cols + (c + j) * 4));
 #pragma unroll
-            for (int j = 0; j < STEP; j += 4) {
-              const uint32_t(&q)[STEP] = r[c & 1];
-              // (volatile: in order with the reads of tensor memory, not all ahead of them in registers)
-              f32x2 s0, s1;
-              asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
-                           : "=l"(s0), "=l"(s1)
-                           : "r"(scale + (c * STEP + j) * 4));
-              if (!UNIFORM) {
-                s0 = mul2(s0, ls);
-                s1 = mul2(s1, ls);
-              }
-              // (one value at a time: pairing what tensor memory gives costs more moves than it saves)
-              float t0, t1, t2, t3;
-              unpack2(s0, t0, t1);
-              unpack2(s1, t2, t3);
-              float *o = v + c * STEP + j;
-              o[0] = fmaf(__uint_as_float(q[j]), t0, o[0]);
-              o[1] = fmaf(__uint_as_float(q[j + 1]), t1, o[1]);
-              o[2] = fmaf(__uint_as_float(q[j + 2]), t2, o[2]);
-              o[3] = fmaf(__uint_as_float(q[j + 3]), t3, o[3]);
-            }
-            if (c + 1 < STEPS) wait(r[(c + 1) & 1]);
+            for (int u = 0; u < 4; u++) v[c + j + u] = fmaf(__uint_as_float(r[j + u]), s[u] * ls, v[c + j + u]);
           }
         }
         sums.release();
-        if (g + 1 == AHEAD || b + 1 == p.o.kb) {
-          if (lane == 0) mbar_arrive(bar + 2);
-          group++;
-        }
+        scales.done(b, o.kb);
       }
       const PairItem w = item(p, i);
-      const Operands &o = p.o;
       const uint64_t n = (uint64_t)w.a_row + rank * 128 + quad * 32 + lane;   // b's row
       const uint64_t m0 = (uint64_t)w.b_row + half * COLS;                    // a's first row
       if (n >= o.n) continue;
@@ -431,18 +433,198 @@ struct BlocksOp {
   }
 };
 
-template <int COLS, bool UNIFORM, typename T>
-cudaError_t launch_tiles(const Operands &o, T *out, int sms, cudaStream_t st) {
-  using Op = BlocksOp<COLS, UNIFORM, T>;
-  typename Op::Args args = {};
-  args.bn = 2 * COLS;
-  args.mt = (uint32_t)((o.m + 2 * COLS - 1) / (2 * COLS));
-  args.nt = (uint32_t)((o.n + 255) / 256);
+// More rows: tiles of 256 of a's rows x 256 of b's (128 a thread's warp), bound
+// by the epilogue's 128 x 256 multiply-adds a CTA each K block (256 of the 512
+// clocks that the block's products take, if nothing else were in the way).
+// b's scales square (UNIFORM): a lane is one of a's rows and has one scale a
+// block. Else each value has a scale of its own; columns' scales read by every
+// lane would fill the shared-memory port (128 floats a warp at 16 bytes a
+// clock), so the lanes read tensor memory in 8 x 4 patches, where a thread has
+// 4 rows and 32 columns: 20 reads instead of 32, each of distinct values.
+template <bool UNIFORM, typename T>
+struct WideOp {
+  static constexpr PairKind KIND = PAIR_E4M3;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  using Scales = ScaleStage<128, UNIFORM ? 2 : 256>;
+  static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024;
+  static constexpr int SCRATCH = SCALE_BYTES + kPairEpiWarps * kBoxBytes;
+  using Args = BlocksArgs<T>;
+  static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
+  static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
+    return {(int32_t)((i % p.mt) * 256), (int32_t)((i / p.mt) * 256), 0, p.o.kb, 0};
+  }
+  static __device__ __forceinline__ void init(uint8_t *scratch) { Scales{scratch}.init(); }
+  static __device__ __forceinline__ void help(const Args &p, uint8_t *scratch, uint32_t rank, uint32_t cluster,
+                                              uint32_t clusters, volatile uint32_t *abort) {
+    const Operands &o = p.o;
+    Scales scales{scratch};
+    const bool vec = scales_vec(o);
+    for (uint32_t i = cluster; i < items(p); i += clusters) {
+      const PairItem w = item(p, i);
+      const uint64_t m0 = (uint64_t)w.a_row + rank * 128, n0 = (uint64_t)w.b_row;
+      if (!scales.fill(threadIdx.x - 320,
+                       [&](uint32_t c) {
+                         if (c < 128) return o.a_scales + (min(m0 + c, o.m - 1) >> o.a_shift) * o.kb;
+                         const uint64_t n = n0 + (UNIFORM ? (c - 128) * 128 : c - 128);
+                         return o.b_scales + (min(n, o.n - 1) >> o.b_shift) * o.kb;
+                       },
+                       o.kb, vec, abort))
+        return;
+    }
+  }
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+                                                  uint32_t cluster, uint32_t clusters) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
+    const Operands &o = p.o;
+    Scales scales{scratch};
+    BoxStore box{scratch + SCALE_BYTES + warp * kBoxBytes};
+    for (uint32_t i = cluster; i < items(p); i += clusters) {
+      // UNIFORM: v[c] column c of the lane's row. Else v[32 q + 4 g + u], q = 2 h + l: rows 16 l + lane / 4 (u < 2)
+      // and + 8, columns 64 h + 8 g + 2 (lane % 4) + u % 2
+      float v[128];
+#pragma unroll
+      for (int j = 0; j < 128; j++) v[j] = 0.0f;
+#pragma unroll 1
+      for (uint32_t b = 0; b < o.kb; b++) {
+        const uint32_t scale = scales.take(b, sums);
+        const uint32_t addr = sums.acquire() + half * 128;
+        constexpr int DEEP = UNIFORM ? 2 : 1;   // reads ahead, where registers allow
+        uint32_t r[DEEP][32];
+        auto read = [&](int c, uint32_t(&to)[32]) {
+          if constexpr (UNIFORM) TMEM_LD32(addr + c * 32, to);
+          else TMEM_LD_16X64(addr + (c >> 1) * 64 + ((uint32_t)(c & 1) << 20), to);
+        };
+        if (sums.ok) {
+          read(0, r[0]);
+          float rows[4];
+          if (UNIFORM) {
+            rows[0] = shared_float(scale + (quad * 32 + lane) * 4) * shared_float(scale + (128 + half) * 4);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) rows[u] = shared_float(scale + (quad * 32 + 8 * u + lane / 4) * 4);
+          }
+          tmem_ld_wait();
+          TMEM_KEEP32(r[0]);
+          float c0[8], c1[8];   // the columns' scales of a half's 64 columns
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            if (DEEP == 2 && c < 3) read(c + 1, r[(c + 1) % DEEP]);
+            const uint32_t(&t)[32] = r[c % DEEP];
+            if constexpr (UNIFORM) {
+#pragma unroll
+              for (int j = 0; j < 32; j++) v[c * 32 + j] = fmaf(__uint_as_float(t[j]), rows[0], v[c * 32 + j]);
+            } else {
+              if ((c & 1) == 0) {
+#pragma unroll
+                for (int g = 0; g < 8; g++)
+                  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                               : "=f"(c0[g]), "=f"(c1[g])
+                               : "r"(scale + (128 + half * 128 + (c >> 1) * 64 + g * 8 + 2 * (lane & 3)) * 4));
+              }
+#pragma unroll
+              for (int g = 0; g < 8; g++) {
+                float *o4 = v + c * 32 + g * 4;
+                const float ra = rows[2 * (c & 1)], rb = rows[2 * (c & 1) + 1];
+                o4[0] = fmaf(__uint_as_float(t[4 * g]), ra * c0[g], o4[0]);
+                o4[1] = fmaf(__uint_as_float(t[4 * g + 1]), ra * c1[g], o4[1]);
+                o4[2] = fmaf(__uint_as_float(t[4 * g + 2]), rb * c0[g], o4[2]);
+                o4[3] = fmaf(__uint_as_float(t[4 * g + 3]), rb * c1[g], o4[3]);
+              }
+            }
+            if (c < 3) {
+              if (DEEP == 1) read(c + 1, r[0]);
+              tmem_ld_wait();
+              TMEM_KEEP32(r[(c + 1) % DEEP]);
+            }
+          }
+        }
+        sums.release();
+        scales.done(b, o.kb);
+      }
+      const PairItem w = item(p, i);
+      const uint32_t m0 = (uint32_t)w.a_row + rank * 128 + quad * 32, n0 = (uint32_t)w.b_row + half * 128;
+      if (m0 >= o.m || n0 >= o.n) continue;
+      if (!sums.ok) {
+#pragma unroll
+        for (int j = 0; j < 128; j++) v[j] = __uint_as_float(0x7fc00000u);
+      }
+      if (p.boxes) {
+        constexpr int BOX = 128 / sizeof(T);   // columns of a box
+#pragma unroll
+        for (int x = 0; x < 128 / BOX; x++) {
+          if (n0 + x * BOX >= o.n) break;
+          box.reuse();
+          if constexpr (UNIFORM) {
+            constexpr int V = 16 / sizeof(T);
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+              alignas(16) T t[V];
+#pragma unroll
+              for (int u = 0; u < V; u++) t[u] = from_float<T>(v[x * BOX + c * V + u]);
+              box.put(c, *reinterpret_cast<uint4 *>(t));
+            }
+          } else {
+#pragma unroll
+            for (int g = 0; g < BOX / 8; g++)
+#pragma unroll
+              for (int u = 0; u < 4; u++) {
+                const int col = x * BOX + g * 8;             // of the warp's 128
+                const float *q = v + (2 * (col / 64) + u / 2) * 32 + (col % 64) / 8 * 4 + 2 * (u & 1);
+                const uint32_t row = 8 * u + lane / 4, at = (g * 8 + 2 * (lane & 3)) * sizeof(T);
+                uint8_t *to = box.box + row * 128 + (((at >> 4) ^ (row & 7)) << 4) + (at & 15);
+                alignas(8) T t[2] = {from_float<T>(q[0]), from_float<T>(q[1])};
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<uint2 *>(t);
+                else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<uint32_t *>(t);
+              }
+          }
+          // (in 16-bit values)
+          box.store(&p.map, (int32_t)((n0 + x * BOX) * (sizeof(T) / 2)), (int32_t)m0);
+        }
+      } else {
+        if constexpr (UNIFORM) {
+          if (m0 + lane < o.m) {
+            T *row = p.out + (uint64_t)(m0 + lane) * o.out_stride + n0;
+#pragma unroll
+            for (int j = 0; j < 128; j++)
+              if (n0 + j < o.n) row[j] = from_float<T>(v[j]);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+              const uint32_t m = m0 + 16 * (q & 1) + 8 * (u / 2) + lane / 4;
+              if (m >= o.m) continue;
+#pragma unroll
+              for (int g = 0; g < 8; g++) {
+                const uint32_t n = n0 + 64 * (q / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
+                if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[q * 32 + 4 * g + u]);
+              }
+            }
+        }
+      }
+    }
+  }
+};
+
+template <class Op, typename T>
+cudaError_t launch_tiles(const Operands &o, T *out, bool wide, uint32_t bn, int sms, cudaStream_t st) {
+  BlocksArgs<T> args = {};
+  args.bn = bn;
   args.o = o;
   args.out = out;
-  if (!encode_operand_map(args.a, 1, o.b, o.k, o.n, o.b_stride, 128) ||
-      !encode_operand_map(args.b, 1, o.a, o.k, o.m, o.a_stride, COLS))
-    return cudaErrorInvalidValue;
+  // the tile's 256 rows: a's (wide) or b's; its bn columns: the other's
+  args.mt = (uint32_t)((o.m + (wide ? 256 : bn) - 1) / (wide ? 256 : bn));
+  args.nt = (uint32_t)((o.n + 255) / 256);
+  args.boxes = wide && o.out_stride * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
+               o.n * sizeof(T) / 2 <= 0x7fffffffull;
+  const bool maps =
+      encode_operand_map(args.a, 1, wide ? o.a : o.b, o.k, wide ? o.m : o.n, wide ? o.a_stride : o.b_stride, 128) &&
+      encode_operand_map(args.b, 1, wide ? o.b : o.a, o.k, wide ? o.n : o.m, wide ? o.b_stride : o.a_stride, bn / 2) &&
+      (!args.boxes ||
+       encode_operand_map(&args.map, 2, out, o.n * sizeof(T) / 2, o.m, o.out_stride * sizeof(T), 32));
+  if (!maps) return cudaErrorInvalidValue;
   return launch_pair<Op>(args, args.mt * args.nt, sms, st);
 }
 
@@ -457,11 +639,11 @@ cudaError_t launch_matmul(const Operands &o, T *out, cudaStream_t st) {
   }
   const int sms = op_sms();
   if (sms < 2) return cudaErrorNoDevice;
-  const bool uniform = o.b_shift != 0;
   // columns a thread: the fewest that hold a's rows in one tile
-  if (o.m <= 32) return uniform ? launch_tiles<16, true>(o, out, sms, st) : launch_tiles<16, false>(o, out, sms, st);
-  if (o.m <= 128) return uniform ? launch_tiles<64, true>(o, out, sms, st) : launch_tiles<64, false>(o, out, sms, st);
-  return uniform ? launch_tiles<128, true>(o, out, sms, st) : launch_tiles<128, false>(o, out, sms, st);
+  if (o.m <= 32) return launch_tiles<NarrowOp<16, T>>(o, out, false, 32, sms, st);
+  if (o.m <= 128) return launch_tiles<NarrowOp<64, T>>(o, out, false, 128, sms, st);
+  return o.b_shift ? launch_tiles<WideOp<true, T>>(o, out, true, 256, sms, st)
+                   : launch_tiles<WideOp<false, T>>(o, out, true, 256, sms, st);
 }
 
 }  // namespace
