@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256, M == 1 ? 3 : 2) matmul_few(const Operands
 // each scale row) into one of two buffers, transposed, so that lanes read
 // theirs side by side and columns' can be read several at once.
 //   LANES, COLS: scales a block (COLS 2: one for each half of the columns)
-template <int LANES_, int COLS_>
+template <int EPI, int LANES_, int COLS_>
 struct ScaleStage {
   static constexpr int LANES = LANES_, COLS = COLS_, ROW = LANES + (COLS < 4 ? 4 : COLS), AHEAD = 4;
   static constexpr int BUFFER = AHEAD * ROW * 4;
@@ -266,7 +266,7 @@ struct ScaleStage {
   __device__ __forceinline__ void init() const {   // full[2], empty[2]
     for (int i = 0; i < 2; i++) {
       mbar_init(bars() + i, 2);
-      mbar_init(bars() + 2 + i, kPairEpiWarps);
+      mbar_init(bars() + 2 + i, EPI);
     }
   }
   // The helpers' part for one item: t = 0 .. 63; row(c): scale c's row of kb blocks.
@@ -353,8 +353,8 @@ template <int COLS, typename T>
 struct NarrowOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
-  using Scales = ScaleStage<128, 2 * COLS>;
+  static constexpr int EPI = 8, PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  using Scales = ScaleStage<EPI, 128, 2 * COLS>;
   static constexpr int SCRATCH = Scales::BYTES;
   using Args = BlocksArgs<T>;
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
@@ -370,7 +370,7 @@ struct NarrowOp {
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
       const uint64_t n0 = (uint64_t)w.a_row + rank * 128, m0 = (uint64_t)w.b_row;
-      if (!scales.fill(threadIdx.x - 320,
+      if (!scales.fill(threadIdx.x - 32 * (EPI + 2),
                        [&](uint32_t c) {
                          return c < 128 ? o.b_scales + (min(n0 + c, o.n - 1) >> o.b_shift) * o.kb
                                         : o.a_scales + (min(m0 + c - 128, o.m - 1) >> o.a_shift) * o.kb;
@@ -433,22 +433,22 @@ struct NarrowOp {
   }
 };
 
-// More rows: tiles of 256 of a's rows x 256 of b's (128 a thread's warp), bound
-// by the epilogue's 128 x 256 multiply-adds a CTA each K block (256 of the 512
-// clocks that the block's products take, if nothing else were in the way).
+// More rows: tiles of 256 of a's rows x 256 of b's, 64 columns a thread's warp
+// (16 epilogue warps: with 8 and 128 columns each, a block's scaling took 1,000
+// clocks a warp, mostly latency, against 720 for its loads and products).
 // b's scales square (UNIFORM): a lane is one of a's rows and has one scale a
 // block. Else each value has a scale of its own; columns' scales read by every
-// lane would fill the shared-memory port (128 floats a warp at 16 bytes a
-// clock), so the lanes read tensor memory in 8 x 4 patches, where a thread has
-// 4 rows and 32 columns: 20 reads instead of 32, each of distinct values.
+// lane would fill the shared-memory port (a float4 for all lanes takes two of
+// its clocks), so the lanes read tensor memory in 8 x 4 patches, where a thread
+// has 4 rows and 16 columns: 12 reads instead of 16, each of distinct values.
 template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
-  using Scales = ScaleStage<128, UNIFORM ? 2 : 256>;
-  static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024;
-  static constexpr int SCRATCH = SCALE_BYTES + kPairEpiWarps * kBoxBytes;
+  static constexpr int EPI = 16, PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  using Scales = ScaleStage<EPI, 128, UNIFORM ? 2 : 256>;
+  static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024, BOX_BYTES = 32 * 64;
+  static constexpr int SCRATCH = SCALE_BYTES + EPI * BOX_BYTES;
   using Args = BlocksArgs<T>;
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
@@ -463,7 +463,7 @@ struct WideOp {
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
       const uint64_t m0 = (uint64_t)w.a_row + rank * 128, n0 = (uint64_t)w.b_row;
-      if (!scales.fill(threadIdx.x - 320,
+      if (!scales.fill(threadIdx.x - 32 * (EPI + 2),
                        [&](uint32_t c) {
                          if (c < 128) return o.a_scales + (min(m0 + c, o.m - 1) >> o.a_shift) * o.kb;
                          const uint64_t n = n0 + (UNIFORM ? (c - 128) * 128 : c - 128);
@@ -475,67 +475,56 @@ struct WideOp {
   }
   static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
                                                   uint32_t cluster, uint32_t clusters) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp >> 2, quad = warp & 3;
     const Operands &o = p.o;
     Scales scales{scratch};
-    BoxStore box{scratch + SCALE_BYTES + warp * kBoxBytes};
+    BoxStore<64> box{scratch + SCALE_BYTES + warp * BOX_BYTES};
     for (uint32_t i = cluster; i < items(p); i += clusters) {
-      // UNIFORM: v[c] column c of the lane's row. Else v[32 q + 4 g + u], q = 2 h + l: rows 16 l + lane / 4 (u < 2)
-      // and + 8, columns 64 h + 8 g + 2 (lane % 4) + u % 2
-      float v[128];
+      // UNIFORM: v[c] column c of the lane's row. Else v[16 c + 4 g + u], c = 2 h + l: rows 16 l + lane / 4 (u < 2)
+      // and + 8, columns 32 h + 8 g + 2 (lane % 4) + u % 2
+      float v[64];
 #pragma unroll
-      for (int j = 0; j < 128; j++) v[j] = 0.0f;
+      for (int j = 0; j < 64; j++) v[j] = 0.0f;
 #pragma unroll 1
       for (uint32_t b = 0; b < o.kb; b++) {
         const uint32_t scale = scales.take(b, sums);
-        const uint32_t addr = sums.acquire() + half * 128;
-        constexpr int DEEP = UNIFORM ? 2 : 1;   // reads ahead, where registers allow
-        uint32_t r[DEEP][32];
-        auto read = [&](int c, uint32_t(&to)[32]) {
-          if constexpr (UNIFORM) TMEM_LD32(addr + c * 32, to);
-          else TMEM_LD_16X64(addr + (c >> 1) * 64 + ((uint32_t)(c & 1) << 20), to);
-        };
+        const uint32_t addr = sums.acquire() + quarter * 64;
         if (sums.ok) {
-          read(0, r[0]);
-          float rows[4];
-          if (UNIFORM) {
-            rows[0] = shared_float(scale + (quad * 32 + lane) * 4) * shared_float(scale + (128 + half) * 4);
-          } else {
-#pragma unroll
-            for (int u = 0; u < 4; u++) rows[u] = shared_float(scale + (quad * 32 + 8 * u + lane / 4) * 4);
-          }
-          tmem_ld_wait();
-          TMEM_KEEP32(r[0]);
-          float c0[8], c1[8];   // the columns' scales of a half's 64 columns
+          float s = 0.0f;
+          if constexpr (UNIFORM)
+            s = shared_float(scale + (quad * 32 + lane) * 4) * shared_float(scale + (128 + quarter / 2) * 4);
 #pragma unroll
           for (int c = 0; c < 4; c++) {
-            if (DEEP == 2 && c < 3) read(c + 1, r[(c + 1) % DEEP]);
-            const uint32_t(&t)[32] = r[c % DEEP];
+            uint32_t t[16];
+            if constexpr (UNIFORM) TMEM_LD16(addr + c * 16, t);
+            else TMEM_LD_16X32(addr + (c >> 1) * 32 + ((uint32_t)(c & 1) << 20), t);
             if constexpr (UNIFORM) {
-#pragma unroll
-              for (int j = 0; j < 32; j++) v[c * 32 + j] = fmaf(__uint_as_float(t[j]), rows[0], v[c * 32 + j]);
-            } else {
-              if ((c & 1) == 0) {
-#pragma unroll
-                for (int g = 0; g < 8; g++)
-                  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
-                               : "=f"(c0[g]), "=f"(c1[g])
-                               : "r"(scale + (128 + half * 128 + (c >> 1) * 64 + g * 8 + 2 * (lane & 3)) * 4));
-              }
-#pragma unroll
-              for (int g = 0; g < 8; g++) {
-                float *o4 = v + c * 32 + g * 4;
-                const float ra = rows[2 * (c & 1)], rb = rows[2 * (c & 1) + 1];
-                o4[0] = fmaf(__uint_as_float(t[4 * g]), ra * c0[g], o4[0]);
-                o4[1] = fmaf(__uint_as_float(t[4 * g + 1]), ra * c1[g], o4[1]);
-                o4[2] = fmaf(__uint_as_float(t[4 * g + 2]), rb * c0[g], o4[2]);
-                o4[3] = fmaf(__uint_as_float(t[4 * g + 3]), rb * c1[g], o4[3]);
-              }
-            }
-            if (c < 3) {
-              if (DEEP == 1) read(c + 1, r[0]);
               tmem_ld_wait();
-              TMEM_KEEP32(r[(c + 1) % DEEP]);
+              TMEM_KEEP16(t);
+#pragma unroll
+              for (int j = 0; j < 16; j++) v[c * 16 + j] = fmaf(__uint_as_float(t[j]), s, v[c * 16 + j]);
+            } else {
+              const uint32_t rows = scale + (quad * 32 + 16 * (c & 1) + lane / 4) * 4;
+              const float ra = shared_float(rows), rb = shared_float(rows + 32);
+              f32x2 cols[4];
+#pragma unroll
+              for (int g = 0; g < 4; g++)
+                asm volatile("ld.shared.b64 %0, [%1];"
+                             : "=l"(cols[g])
+                             : "r"(scale + (128 + quarter * 64 + (c >> 1) * 32 + g * 8 + 2 * (lane & 3)) * 4));
+              tmem_ld_wait();
+              TMEM_KEEP16(t);
+#pragma unroll
+              for (int g = 0; g < 4; g++) {
+                float *o4 = v + c * 16 + g * 4;
+                float a0, a1, b0, b1;
+                unpack2(mul2(cols[g], pack2(ra, ra)), a0, a1);
+                unpack2(mul2(cols[g], pack2(rb, rb)), b0, b1);
+                o4[0] = fmaf(__uint_as_float(t[4 * g]), a0, o4[0]);
+                o4[1] = fmaf(__uint_as_float(t[4 * g + 1]), a1, o4[1]);
+                o4[2] = fmaf(__uint_as_float(t[4 * g + 2]), b0, o4[2]);
+                o4[3] = fmaf(__uint_as_float(t[4 * g + 3]), b1, o4[3]);
+              }
             }
           }
         }
@@ -543,22 +532,22 @@ struct WideOp {
         scales.done(b, o.kb);
       }
       const PairItem w = item(p, i);
-      const uint32_t m0 = (uint32_t)w.a_row + rank * 128 + quad * 32, n0 = (uint32_t)w.b_row + half * 128;
+      const uint32_t m0 = (uint32_t)w.a_row + rank * 128 + quad * 32, n0 = (uint32_t)w.b_row + quarter * 64;
       if (m0 >= o.m || n0 >= o.n) continue;
       if (!sums.ok) {
 #pragma unroll
-        for (int j = 0; j < 128; j++) v[j] = __uint_as_float(0x7fc00000u);
+        for (int j = 0; j < 64; j++) v[j] = __uint_as_float(0x7fc00000u);
       }
       if (p.boxes) {
-        constexpr int BOX = 128 / sizeof(T);   // columns of a box
+        constexpr int BOX = 64 / sizeof(T);   // columns of a box
 #pragma unroll
-        for (int x = 0; x < 128 / BOX; x++) {
+        for (int x = 0; x < 64 / BOX; x++) {
           if (n0 + x * BOX >= o.n) break;
           box.reuse();
           if constexpr (UNIFORM) {
             constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
+            for (int c = 0; c < 4; c++) {
               alignas(16) T t[V];
 #pragma unroll
               for (int u = 0; u < V; u++) t[u] = from_float<T>(v[x * BOX + c * V + u]);
@@ -569,10 +558,10 @@ struct WideOp {
             for (int g = 0; g < BOX / 8; g++)
 #pragma unroll
               for (int u = 0; u < 4; u++) {
-                const int col = x * BOX + g * 8;             // of the warp's 128
-                const float *q = v + (2 * (col / 64) + u / 2) * 32 + (col % 64) / 8 * 4 + 2 * (u & 1);
-                const uint32_t row = 8 * u + lane / 4, at = (g * 8 + 2 * (lane & 3)) * sizeof(T);
-                uint8_t *to = box.box + row * 128 + (((at >> 4) ^ (row & 7)) << 4) + (at & 15);
+                const int col = x * BOX + g * 8;             // of the warp's 64
+                const float *q = v + (2 * (col / 32) + u / 2) * 16 + (col % 32) / 8 * 4 + 2 * (u & 1);
+                const uint32_t at = (g * 8 + 2 * (lane & 3)) * sizeof(T);
+                uint8_t *to = box.at(8 * u + lane / 4, at >> 4) + (at & 15);
                 alignas(8) T t[2] = {from_float<T>(q[0]), from_float<T>(q[1])};
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<uint2 *>(t);
                 else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<uint32_t *>(t);
@@ -581,28 +570,26 @@ struct WideOp {
           // (in 16-bit values)
           box.store(&p.map, (int32_t)((n0 + x * BOX) * (sizeof(T) / 2)), (int32_t)m0);
         }
-      } else {
-        if constexpr (UNIFORM) {
-          if (m0 + lane < o.m) {
-            T *row = p.out + (uint64_t)(m0 + lane) * o.out_stride + n0;
+      } else if constexpr (UNIFORM) {
+        if (m0 + lane < o.m) {
+          T *row = p.out + (uint64_t)(m0 + lane) * o.out_stride + n0;
 #pragma unroll
-            for (int j = 0; j < 128; j++)
-              if (n0 + j < o.n) row[j] = from_float<T>(v[j]);
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-              const uint32_t m = m0 + 16 * (q & 1) + 8 * (u / 2) + lane / 4;
-              if (m >= o.m) continue;
-#pragma unroll
-              for (int g = 0; g < 8; g++) {
-                const uint32_t n = n0 + 64 * (q / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
-                if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[q * 32 + 4 * g + u]);
-              }
-            }
+          for (int j = 0; j < 64; j++)
+            if (n0 + j < o.n) row[j] = from_float<T>(v[j]);
         }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const uint32_t m = m0 + 16 * (c & 1) + 8 * (u / 2) + lane / 4;
+            if (m >= o.m) continue;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+              const uint32_t n = n0 + 32 * (c / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
+              if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[c * 16 + 4 * g + u]);
+            }
+          }
       }
     }
   }
@@ -623,7 +610,7 @@ cudaError_t launch_tiles(const Operands &o, T *out, bool wide, uint32_t bn, int 
       encode_operand_map(args.a, 1, wide ? o.a : o.b, o.k, wide ? o.m : o.n, wide ? o.a_stride : o.b_stride, 128) &&
       encode_operand_map(args.b, 1, wide ? o.b : o.a, o.k, wide ? o.n : o.m, wide ? o.b_stride : o.a_stride, bn / 2) &&
       (!args.boxes ||
-       encode_operand_map(&args.map, 2, out, o.n * sizeof(T) / 2, o.m, o.out_stride * sizeof(T), 32));
+       encode_narrow_map(&args.map, out, o.n * sizeof(T) / 2, o.m, o.out_stride * sizeof(T)));
   if (!maps) return cudaErrorInvalidValue;
   return launch_pair<Op>(args, args.mt * args.nt, sms, st);
 }

@@ -39,6 +39,8 @@ inline int op_launched(const char *what, unsigned long long kernels) {
 bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
                         uint64_t pitch, uint32_t box_rows);
 
+// 16-bit values [outer][inner] written in boxes of 64 bytes x 32 rows, 64-byte swizzle (shard.cu).
+bool encode_narrow_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t pitch);
 // FP32 sums [planes][outer][inner] in boxes of 32 values x 32 rows (shard.cu).
 bool encode_sums_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch);
 
