@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pair_gemm.cuh"
 
@@ -255,9 +256,14 @@ __global__ void __launch_bounds__(256, M == 1 ? 3 : 2) matmul_few(const Operands
 // each scale row) into one of two buffers, transposed, so that lanes read
 // theirs side by side and columns' can be read several at once.
 //   LANES, COLS: scales a block (COLS 2: one for each half of the columns)
-template <int EPI, int LANES_, int COLS_>
+//   Order: where scale c of a block is kept, of ROW floats
+struct InOrder {
+  static constexpr int room(int n) { return n; }
+  static __device__ __forceinline__ uint32_t place(uint32_t c) { return c; }
+};
+template <int LANES_, int COLS_, typename Order = InOrder>
 struct ScaleStage {
-  static constexpr int LANES = LANES_, COLS = COLS_, ROW = LANES + (COLS < 4 ? 4 : COLS), AHEAD = 4;
+  static constexpr int LANES = LANES_, COLS = COLS_, ROW = Order::room(LANES + (COLS < 4 ? 4 : COLS)), AHEAD = 4;
   static constexpr int BUFFER = AHEAD * ROW * 4;
   static constexpr int BYTES = 2 * BUFFER + 64;
   uint8_t *scratch;
@@ -266,7 +272,7 @@ struct ScaleStage {
   __device__ __forceinline__ void init() const {   // full[2], empty[2]
     for (int i = 0; i < 2; i++) {
       mbar_init(bars() + i, 2);
-      mbar_init(bars() + 2 + i, EPI);
+      mbar_init(bars() + 2 + i, kPairEpi);
     }
   }
   // The helpers' part for one item: t = 0 .. 63; row(c): scale c's row of kb blocks.
@@ -297,12 +303,12 @@ struct ScaleStage {
       float *at = reinterpret_cast<float *>(scratch + (group & 1) * BUFFER);
 #pragma unroll
       for (int e = 0; e < EACH; e++) {
-        const uint32_t c = t + 64 * e;
+        const uint32_t c = t + 64 * e, to = Order::place(c);
         if (c < LANES + COLS) {
-          at[c] = v[e].x;
-          at[ROW + c] = v[e].y;
-          at[2 * ROW + c] = v[e].z;
-          at[3 * ROW + c] = v[e].w;
+          at[to] = v[e].x;
+          at[ROW + to] = v[e].y;
+          at[2 * ROW + to] = v[e].z;
+          at[3 * ROW + to] = v[e].w;
         }
       }
       __syncwarp();
@@ -353,8 +359,8 @@ template <int COLS, typename T>
 struct NarrowOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int EPI = 8, PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
-  using Scales = ScaleStage<EPI, 128, 2 * COLS>;
+  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  using Scales = ScaleStage<128, 2 * COLS>;
   static constexpr int SCRATCH = Scales::BYTES;
   using Args = BlocksArgs<T>;
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
@@ -370,7 +376,7 @@ struct NarrowOp {
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
       const uint64_t n0 = (uint64_t)w.a_row + rank * 128, m0 = (uint64_t)w.b_row;
-      if (!scales.fill(threadIdx.x - 32 * (EPI + 2),
+      if (!scales.fill(threadIdx.x - 32 * (kPairEpi + 2),
                        [&](uint32_t c) {
                          return c < 128 ? o.b_scales + (min(n0 + c, o.n - 1) >> o.b_shift) * o.kb
                                         : o.a_scales + (min(m0 + c - 128, o.m - 1) >> o.a_shift) * o.kb;
@@ -433,22 +439,35 @@ struct NarrowOp {
   }
 };
 
-// More rows: tiles of 256 of a's rows x 256 of b's, 64 columns a thread's warp
-// (16 epilogue warps: with 8 and 128 columns each, a block's scaling took 1,000
-// clocks a warp, mostly latency, against 720 for its loads and products).
+// Scales for lanes that hold 8 x 4 patches (below): a thread's 4 rows side by
+// side, then each half's columns, a thread's 32 side by side (4 threads of a row
+// 36 floats apart: different banks).
+struct PatchOrder {
+  static constexpr int room(int) { return 128 + 2 * 4 * 36; }
+  static __device__ __forceinline__ uint32_t place(uint32_t c) {
+    if (c < 128) return (c & ~31u) + (c & 7) * 4 + ((c >> 3) & 3);
+    c -= 128;
+    return 128 + (c >> 7) * 144 + ((c >> 1) & 3) * 36 + ((c & 127) >> 3) * 2 + (c & 1);
+  }
+};
+__device__ __forceinline__ void shared_float4(uint32_t addr, float (&v)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr));
+}
+
+// More rows: tiles of 256 of a's rows x 256 of b's, 128 columns a thread's warp.
 // b's scales square (UNIFORM): a lane is one of a's rows and has one scale a
 // block. Else each value has a scale of its own; columns' scales read by every
-// lane would fill the shared-memory port (a float4 for all lanes takes two of
-// its clocks), so the lanes read tensor memory in 8 x 4 patches, where a thread
-// has 4 rows and 16 columns: 12 reads instead of 16, each of distinct values.
+// lane would fill the shared-memory port, so the lanes read tensor memory in 8 x
+// 4 patches, where a thread has 4 rows and 32 columns: 9 reads of shared memory
+// a block.
 template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int EPI = 16, PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
-  using Scales = ScaleStage<EPI, 128, UNIFORM ? 2 : 256>;
-  static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024, BOX_BYTES = 32 * 64;
-  static constexpr int SCRATCH = SCALE_BYTES + EPI * BOX_BYTES;
+  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  using Scales = ScaleStage<128, UNIFORM ? 2 : 256, std::conditional_t<UNIFORM, InOrder, PatchOrder>>;
+  static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024;
+  static constexpr int SCRATCH = SCALE_BYTES + kPairEpi * kBoxBytes;
   using Args = BlocksArgs<T>;
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
@@ -463,7 +482,7 @@ struct WideOp {
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
       const uint64_t m0 = (uint64_t)w.a_row + rank * 128, n0 = (uint64_t)w.b_row;
-      if (!scales.fill(threadIdx.x - 32 * (EPI + 2),
+      if (!scales.fill(threadIdx.x - 32 * (kPairEpi + 2),
                        [&](uint32_t c) {
                          if (c < 128) return o.a_scales + (min(m0 + c, o.m - 1) >> o.a_shift) * o.kb;
                          const uint64_t n = n0 + (UNIFORM ? (c - 128) * 128 : c - 128);
@@ -475,56 +494,69 @@ struct WideOp {
   }
   static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
                                                   uint32_t cluster, uint32_t clusters) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp >> 2, quad = warp & 3;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
     const Operands &o = p.o;
     Scales scales{scratch};
-    BoxStore<64> box{scratch + SCALE_BYTES + warp * BOX_BYTES};
+    BoxStore box{scratch + SCALE_BYTES + warp * kBoxBytes};
     for (uint32_t i = cluster; i < items(p); i += clusters) {
-      // UNIFORM: v[c] column c of the lane's row. Else v[16 c + 4 g + u], c = 2 h + l: rows 16 l + lane / 4 (u < 2)
-      // and + 8, columns 32 h + 8 g + 2 (lane % 4) + u % 2
-      float v[64];
+      // UNIFORM: v[c] column c of the lane's row. Else v[32 c + 4 g + u], c = 2 h + l: rows 16 l + lane / 4 (u < 2)
+      // and + 8, columns 64 h + 8 g + 2 (lane % 4) + u % 2
+      float v[128];
 #pragma unroll
-      for (int j = 0; j < 64; j++) v[j] = 0.0f;
+      for (int j = 0; j < 128; j++) v[j] = 0.0f;
 #pragma unroll 1
       for (uint32_t b = 0; b < o.kb; b++) {
         const uint32_t scale = scales.take(b, sums);
-        const uint32_t addr = sums.acquire() + quarter * 64;
+        const uint32_t addr = sums.acquire() + half * 128;
         if (sums.ok) {
-          float s = 0.0f;
+          constexpr int DEEP = UNIFORM ? 2 : 1;   // reads ahead, where registers allow
+          uint32_t r[DEEP][32];
+          auto read = [&](int c, uint32_t(&to)[32]) {
+            if constexpr (UNIFORM) TMEM_LD32(addr + c * 32, to);
+            else TMEM_LD_16X64(addr + (c >> 1) * 64 + ((uint32_t)(c & 1) << 20), to);
+          };
+          read(0, r[0]);
+          float rows[4];
+          f32x2 cols[8];
           if constexpr (UNIFORM)
-            s = shared_float(scale + (quad * 32 + lane) * 4) * shared_float(scale + (128 + quarter / 2) * 4);
+            rows[0] = shared_float(scale + (quad * 32 + lane) * 4) * shared_float(scale + (128 + half) * 4);
+          else shared_float4(scale + (quad * 32 + (lane >> 2) * 4) * 4, rows);
+          tmem_ld_wait();
+          TMEM_KEEP32(r[0]);
 #pragma unroll
           for (int c = 0; c < 4; c++) {
-            uint32_t t[16];
-            if constexpr (UNIFORM) TMEM_LD16(addr + c * 16, t);
-            else TMEM_LD_16X32(addr + (c >> 1) * 32 + ((uint32_t)(c & 1) << 20), t);
+            if (DEEP == 2 && c < 3) read(c + 1, r[(c + 1) % DEEP]);
+            const uint32_t(&t)[32] = r[c % DEEP];
             if constexpr (UNIFORM) {
-              tmem_ld_wait();
-              TMEM_KEEP16(t);
 #pragma unroll
-              for (int j = 0; j < 16; j++) v[c * 16 + j] = fmaf(__uint_as_float(t[j]), s, v[c * 16 + j]);
+              for (int j = 0; j < 32; j++) v[c * 32 + j] = fmaf(__uint_as_float(t[j]), rows[0], v[c * 32 + j]);
             } else {
-              const uint32_t rows = scale + (quad * 32 + 16 * (c & 1) + lane / 4) * 4;
-              const float ra = shared_float(rows), rb = shared_float(rows + 32);
-              f32x2 cols[4];
+              if ((c & 1) == 0) {   // 64 columns' scales: 16 a thread
 #pragma unroll
-              for (int g = 0; g < 4; g++)
-                asm volatile("ld.shared.b64 %0, [%1];"
-                             : "=l"(cols[g])
-                             : "r"(scale + (128 + quarter * 64 + (c >> 1) * 32 + g * 8 + 2 * (lane & 3)) * 4));
-              tmem_ld_wait();
-              TMEM_KEEP16(t);
+                for (int k = 0; k < 4; k++) {
+                  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
+                               : "=l"(cols[2 * k]), "=l"(cols[2 * k + 1])
+                               : "r"(scale + (128 + half * 144 + (lane & 3) * 36 + (c >> 1) * 16 + 4 * k) * 4));
+                }
+              }
+              const f32x2 ra = pack2(rows[2 * (c & 1)], rows[2 * (c & 1)]);
+              const f32x2 rb = pack2(rows[2 * (c & 1) + 1], rows[2 * (c & 1) + 1]);
 #pragma unroll
-              for (int g = 0; g < 4; g++) {
-                float *o4 = v + c * 16 + g * 4;
+              for (int g = 0; g < 8; g++) {
+                float *o4 = v + c * 32 + g * 4;
                 float a0, a1, b0, b1;
-                unpack2(mul2(cols[g], pack2(ra, ra)), a0, a1);
-                unpack2(mul2(cols[g], pack2(rb, rb)), b0, b1);
+                unpack2(mul2(cols[g], ra), a0, a1);
+                unpack2(mul2(cols[g], rb), b0, b1);
                 o4[0] = fmaf(__uint_as_float(t[4 * g]), a0, o4[0]);
                 o4[1] = fmaf(__uint_as_float(t[4 * g + 1]), a1, o4[1]);
                 o4[2] = fmaf(__uint_as_float(t[4 * g + 2]), b0, o4[2]);
                 o4[3] = fmaf(__uint_as_float(t[4 * g + 3]), b1, o4[3]);
               }
+            }
+            if (c < 3) {
+              if (DEEP == 1) read(c + 1, r[0]);
+              tmem_ld_wait();
+              TMEM_KEEP32(r[(c + 1) % DEEP]);
             }
           }
         }
@@ -532,40 +564,50 @@ struct WideOp {
         scales.done(b, o.kb);
       }
       const PairItem w = item(p, i);
-      const uint32_t m0 = (uint32_t)w.a_row + rank * 128 + quad * 32, n0 = (uint32_t)w.b_row + quarter * 64;
+      const uint32_t m0 = (uint32_t)w.a_row + rank * 128 + quad * 32, n0 = (uint32_t)w.b_row + half * 128;
       if (m0 >= o.m || n0 >= o.n) continue;
       if (!sums.ok) {
 #pragma unroll
-        for (int j = 0; j < 64; j++) v[j] = __uint_as_float(0x7fc00000u);
+        for (int j = 0; j < 128; j++) v[j] = __uint_as_float(0x7fc00000u);
       }
       if (p.boxes) {
-        constexpr int BOX = 64 / sizeof(T);   // columns of a box
+        constexpr int BOX = 128 / sizeof(T);   // columns of a box
 #pragma unroll
-        for (int x = 0; x < 64 / BOX; x++) {
+        for (int x = 0; x < 128 / BOX; x++) {
           if (n0 + x * BOX >= o.n) break;
           box.reuse();
           if constexpr (UNIFORM) {
             constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-              alignas(16) T t[V];
-#pragma unroll
-              for (int u = 0; u < V; u++) t[u] = from_float<T>(v[x * BOX + c * V + u]);
-              box.put(c, *reinterpret_cast<uint4 *>(t));
+            for (int c = 0; c < 8; c++) {
+              box.put(c, pack_chunk(v + x * BOX + c * V, static_cast<T *>(nullptr)));
             }
           } else {
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int g = 0; g < BOX / 8; g++)
+              for (int g = 0; g < 4; g++)
 #pragma unroll
-              for (int u = 0; u < 4; u++) {
-                const int col = x * BOX + g * 8;             // of the warp's 64
-                const float *q = v + (2 * (col / 32) + u / 2) * 16 + (col % 32) / 8 * 4 + 2 * (u & 1);
-                const uint32_t at = (g * 8 + 2 * (lane & 3)) * sizeof(T);
-                uint8_t *to = box.at(8 * u + lane / 4, at >> 4) + (at & 15);
-                alignas(8) T t[2] = {from_float<T>(q[0]), from_float<T>(q[1])};
-                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<uint2 *>(t);
-                else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<uint32_t *>(t);
+                for (int u = 0; u < 4; u++) {
+                  const float *q = v + (2 * (x / 2) + u / 2) * 32 + ((x & 1) * 4 + g) * 4 + 2 * (u & 1);
+                  const uint32_t at = (g * 8 + 2 * (lane & 3)) * 4;
+                  *reinterpret_cast<float2 *>(box.at(8 * u + lane / 4, at >> 4) + (at & 15)) = make_float2(q[0], q[1]);
+                }
+            } else {
+              // 8 x 8 patches, four (a column of the box's 32 rows) at a time: lane l gives the address of row l
+#pragma unroll
+              for (int g = 0; g < 8; g++) {
+                uint32_t q[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                  const float *w2 = v + (2 * x + u / 2) * 32 + g * 4 + 2 * (u & 1);
+                  q[u] = pack16<T>(w2[0], w2[1]);
+                }
+                asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                                 smem_u32(box.at(lane, g))),
+                             "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                             : "memory");
               }
+            }
           }
           // (in 16-bit values)
           box.store(&p.map, (int32_t)((n0 + x * BOX) * (sizeof(T) / 2)), (int32_t)m0);
@@ -574,7 +616,7 @@ struct WideOp {
         if (m0 + lane < o.m) {
           T *row = p.out + (uint64_t)(m0 + lane) * o.out_stride + n0;
 #pragma unroll
-          for (int j = 0; j < 64; j++)
+          for (int j = 0; j < 128; j++)
             if (n0 + j < o.n) row[j] = from_float<T>(v[j]);
         }
       } else {
@@ -585,9 +627,9 @@ struct WideOp {
             const uint32_t m = m0 + 16 * (c & 1) + 8 * (u / 2) + lane / 4;
             if (m >= o.m) continue;
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-              const uint32_t n = n0 + 32 * (c / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
-              if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[c * 16 + 4 * g + u]);
+            for (int g = 0; g < 8; g++) {
+              const uint32_t n = n0 + 64 * (c / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
+              if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[c * 32 + 4 * g + u]);
             }
           }
       }
@@ -610,7 +652,7 @@ cudaError_t launch_tiles(const Operands &o, T *out, bool wide, uint32_t bn, int 
       encode_operand_map(args.a, 1, wide ? o.a : o.b, o.k, wide ? o.m : o.n, wide ? o.a_stride : o.b_stride, 128) &&
       encode_operand_map(args.b, 1, wide ? o.b : o.a, o.k, wide ? o.n : o.m, wide ? o.b_stride : o.a_stride, bn / 2) &&
       (!args.boxes ||
-       encode_narrow_map(&args.map, out, o.n * sizeof(T) / 2, o.m, o.out_stride * sizeof(T)));
+       encode_operand_map(&args.map, 2, out, o.n * sizeof(T) / 2, o.m, o.out_stride * sizeof(T), 32));
   if (!maps) return cudaErrorInvalidValue;
   return launch_pair<Op>(args, args.mt * args.nt, sms, st);
 }

@@ -178,7 +178,7 @@ template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
 struct LogitsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? EPI * kBoxBytes : 0, MAX_STAGES = 8;
+  static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? kPairEpi * kBoxBytes : 0, MAX_STAGES = 8;
   static constexpr int CHUNK = PLANES == 2 ? 2 : 6;   // 24 steps of the tensor cores
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];
@@ -227,7 +227,7 @@ struct LogitsOp : PairNoHelpers {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const double scale2 = PLANES == 2 ? p.scale2 * (double)undo_scale(p.maxima[MAX_ROWS]) : p.scale2;
     const float unit = GRAD ? grad_unit(p.maxima[MAX_GRAD]) : 1.0f;
-    BoxStore<> box{scratch + warp * kBoxBytes};
+    BoxStore box{scratch + warp * kBoxBytes};
     Row next = row_of(p, cluster, rank);
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
@@ -407,7 +407,7 @@ template <PairKind KIND_, int PLANES_>
 struct QueriesOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = true;
-  static constexpr int PLANES = PLANES_, SCRATCH = EPI * kBoxBytes, MAX_STAGES = 8;
+  static constexpr int PLANES = PLANES_, SCRATCH = kPairEpi * kBoxBytes, MAX_STAGES = 8;
   static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); W's rows from the piece's first on
@@ -439,7 +439,7 @@ struct QueriesOp : PairNoHelpers {
     uint32_t tmem = 0;
     if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
     else tmem = sums.acquire() + half * cols;
-    BoxStore<> box{scratch + warp * kBoxBytes};
+    BoxStore box{scratch + warp * kBoxBytes};
 #pragma unroll
     for (uint32_t c = 0; c < 4; c++) {
       const uint32_t d0 = (uint32_t)w.b_row + half * cols + c * 32;
@@ -470,7 +470,7 @@ template <PairKind KIND_, int PLANES_, typename T>
 struct RowsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = true, B_MN = true;
-  static constexpr int PLANES = PLANES_, SCRATCH = EPI * kBoxBytes, MAX_STAGES = 8;
+  static constexpr int PLANES = PLANES_, SCRATCH = kPairEpi * kBoxBytes, MAX_STAGES = 8;
   static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); X
@@ -504,7 +504,7 @@ struct RowsOp : PairNoHelpers {
     if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
     else tmem = sums.acquire() + half * cols;
     T *row = p.out + (uint64_t)i * p.dims;
-    BoxStore<> box{scratch + warp * kBoxBytes};
+    BoxStore box{scratch + warp * kBoxBytes};
     constexpr uint32_t BOX = 128 / sizeof(T), V = 16 / sizeof(T);   // values of a box row, of a chunk
 #pragma unroll
     for (uint32_t c = 0; c < 4; c++) {

@@ -23,6 +23,24 @@ template <> __device__ __forceinline__ float from_float<float>(float x) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Two values rounded to a 16-bit type, packed.
+template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 16 bytes of T from FP32.
+__device__ __forceinline__ uint4 pack_chunk(const float *v, float *) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <typename T> __device__ __forceinline__ uint4 pack_chunk(const float *v, T *) {
+  return make_uint4(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]), pack16<T>(v[6], v[7]));
+}
+
 inline bool op_dtype(uint32_t dtype) { return dtype == ANNB200_F32 || dtype == ANNB200_F16 || dtype == ANNB200_BF16; }
 inline uint32_t op_bytes(uint32_t dtype) { return dtype == ANNB200_F32 ? 4 : 2; }
 
@@ -39,8 +57,6 @@ inline int op_launched(const char *what, unsigned long long kernels) {
 bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
                         uint64_t pitch, uint32_t box_rows);
 
-// 16-bit values [outer][inner] written in boxes of 64 bytes x 32 rows, 64-byte swizzle (shard.cu).
-bool encode_narrow_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t pitch);
 // FP32 sums [planes][outer][inner] in boxes of 32 values x 32 rows (shard.cu).
 bool encode_sums_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch);
 

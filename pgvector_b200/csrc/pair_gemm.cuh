@@ -9,13 +9,12 @@
 // list. Roles in each CTA:
 //
 //   warps 0-7  epilogue: warp w reads tensor memory lanes 32 (w % 4) .. + 31
-//   (or 0-15)  and columns of the half (quarter) w / 4, so a thread holds half
-//              (a quarter of) a row. The next four:
-//   first      TMA producer: the CTA's own tiles of each 128-byte K block, all
+//              and columns of the half w / 4, so a thread holds half a row.
+//   warp 8     TMA producer: the CTA's own tiles of each 128-byte K block, all
 //              completing on the leader CTA's barrier.
-//   second     MMA issuer (leader CTA); tcgen05.commit frees the stage and
+//   warp 9     MMA issuer (leader CTA); tcgen05.commit frees the stage and
 //              publishes the sums in both CTAs.
-//   two more   an operator's helpers, if it has any.
+//   10 and 11  an operator's helpers, if it has any.
 //
 // Two sums of 256 columns each let the epilogue of one run under the products
 // of the next. The tensor cores cut off, and do not round, what falls below a
@@ -38,16 +37,13 @@
 
 namespace annb200 {
 
-// Threads and registers: an operator's EPI epilogue warps (8, or 16 where a
-// thread's share of a tile must be smaller) and 4 more. The kernel starts with
-// 168 (96) registers a thread; the epilogue's go up to 224 (104) and the
-// others' down to 56, each side at the top of its own branch, which no other
-// joins. Together they take no more than the block started with.
-template <class Op> constexpr int pair_threads() { return 32 * (Op::EPI + 4); }
-template <class Op> constexpr int pair_epi_regs() { return Op::EPI == 8 ? 224 : 104; }
-constexpr int kPairOtherRegs = 56;
-static_assert(256 * 224 + 128 * kPairOtherRegs <= 384 * 168, "more registers than the block starts with");
-static_assert(512 * 104 + 128 * kPairOtherRegs <= 640 * 96, "more registers than the block starts with");
+constexpr int kPairEpi = 8;                          // epilogue warps
+constexpr int kPairThreads = 32 * (kPairEpi + 4);    // whole warpgroups, for the register split
+// Registers a thread: 384 threads start with 168 each. The epilogue's 256 go up
+// to 224 and the other 128 down to 56, each side at the top of its own branch,
+// which no other joins. Together they take no more than the block started with.
+constexpr int kPairEpiRegs = 224, kPairOtherRegs = 56;
+static_assert(256 * kPairEpiRegs + 128 * kPairOtherRegs <= 384 * 168, "more registers than the block starts with");
 constexpr int kPairTileBytes = 128 * 128;     // 128 rows of 128 bytes (or 128 bytes wide, 128 K rows)
 constexpr int kPairSmem = 227 * 1024;
 
@@ -156,12 +152,11 @@ __device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volati
 // conflicts) and stored as one box by the TMA, whole lines at a time. Rows and
 // columns past the tensor's ends are left out by the TMA.
 constexpr int kBoxBytes = 32 * 128;
-template <int WIDTH = 128>   // bytes of a row; 64: 64-byte swizzle
 struct BoxStore {
   uint8_t *box;
-  // 16-byte chunk of a row
+  // A row's 16-byte chunk.
   __device__ __forceinline__ uint8_t *at(uint32_t row, uint32_t chunk) const {
-    return box + row * WIDTH + ((WIDTH == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
+    return box + row * 128 + ((chunk ^ (row & 7)) << 4);
   }
   // Before the box is filled again: what was stored from it has been read.
   __device__ __forceinline__ void reuse() {
@@ -290,13 +285,13 @@ struct PairShape {
   static constexpr int smem(int b_bytes) { return 1024 + stages(b_bytes) * stage(b_bytes) + BAR_BYTES + Op::SCRATCH; }
 };
 
-// Op: EPI (epilogue warps), KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
+// Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
 // sum; 0: the item's), HELPERS (0 or 2 warps), Args with maps a[PLANES],
 // b[PLANES] and bn (columns of a tile), items(args), item(args, i),
 // epilogue(args, sums, scratch, rank, cluster, clusters): all of the cluster's
 // items; init and help where there are helpers.
 struct PairNoHelpers {
-  static constexpr int EPI = 8, HELPERS = 0;
+  static constexpr int HELPERS = 0;
   static __device__ __forceinline__ void init(uint8_t *) {}
   template <class Args>
   static __device__ __forceinline__ void help(const Args &, uint8_t *, uint32_t, uint32_t, uint32_t,
@@ -304,7 +299,7 @@ struct PairNoHelpers {
 };
 
 template <class Op>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<Op>(), 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_gemm(const __grid_constant__ typename Op::Args args) {
   using Shape = PairShape<Op>;
   constexpr int PLANES = Op::PLANES;
@@ -337,13 +332,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<Op>(), 
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(tfull + b, 1);
-      mbar_init(tempty + b, 2 * Op::EPI);
+      mbar_init(tempty + b, 2 * kPairEpi);
     }
     mbar_init(drain, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == Op::EPI + 1) {
+  if (warp == kPairEpi + 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512)
                  : "memory");
@@ -355,14 +350,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<Op>(), 
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp < Op::EPI) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pair_epi_regs<Op>()));
+  if (warp < kPairEpi) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpiRegs));
     PairSums sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
     Op::epilogue(args, sums, scratch, rank, cluster, clusters);
-    BoxStore<>::finish();
+    BoxStore::finish();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairOtherRegs));
-    if (warp == Op::EPI) {
+    if (warp == kPairEpi) {
       if (lane == 0) {
         uint32_t s = 0, round = 0;
         bool ok = true;
@@ -401,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<Op>(), 
         }
       }
       __syncwarp();
-    } else if (warp == Op::EPI + 1) {
+    } else if (warp == kPairEpi + 1) {
       if (lane == 0 && rank == 0) {
         const uint32_t idesc = pair_idesc<Op::KIND, Op::A_MN, Op::B_MN>(args.bn);
         constexpr uint32_t A_STEP = Op::A_MN ? 2048 : 32, B_STEP = Op::B_MN ? 2048 : 32;
@@ -472,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<Op>(), 
   tc_fence_before();
   __syncthreads();
   cluster_sync();
-  if (warp == Op::EPI + 1) {
+  if (warp == kPairEpi + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
@@ -495,7 +490,7 @@ cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, 
     set.fetch_or(bit, std::memory_order_relaxed);
   }
   const uint32_t clusters = items < (uint32_t)(sms / 2) ? items : (uint32_t)(sms / 2);
-  pair_gemm<Op><<<2 * clusters, pair_threads<Op>(), smem, st>>>(args);
+  pair_gemm<Op><<<2 * clusters, kPairThreads, smem, st>>>(args);
   return cudaGetLastError();
 }
 

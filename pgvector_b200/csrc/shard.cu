@@ -446,18 +446,6 @@ bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint
   return bytes == 1 ? encode_u8_seg_map(map, base, inner, outer, pitch, box_rows)
                     : encode_f16_map(map, base, inner, outer, pitch, box_rows);
 }
-// The same tensor written in 64-byte-swizzled boxes of 64 bytes x 32 rows.
-bool encode_narrow_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t pitch) {
-  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {pitch};
-  cuuint32_t box[2] = {32, 32};
-  cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
-         CUDA_SUCCESS;
-}
 // FP32 sums [planes][outer][inner], pitch bytes a row, written and added to in
 // swizzled boxes of 32 values x 32 rows of one plane.
 bool encode_sums_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch) {
