@@ -30,73 +30,116 @@ __device__ __forceinline__ float block_scale(uint32_t bits, float &inverse) {
 }
 
 // 8 values of a row from column c on (c % 8 == 0), zero past k. vec: rows are 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load8(const T *row, uint32_t c, uint32_t k, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= k) {
-    alignas(16) T t[8];
+template <typename T> struct Eight {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *row, uint32_t c, uint32_t k, bool vec) {
+    if (vec && c + 8 <= k) {
 #pragma unroll
-    for (int j = 0; j < (int)(8 * sizeof(T) / 16); j++)
-      reinterpret_cast<uint4 *>(t)[j] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + j);
+      for (int j = 0; j < (int)sizeof(T) / 2; j++) w[j] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + j);
+    } else {
+      T t[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = to_float(t[j]);
-  } else {
+      for (int j = 0; j < 8; j++) t[j] = c + j < k ? row[c + j] : from_float<T>(0.0f);
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = c + j < k ? to_float(row[c + j]) : 0.0f;
+      for (int j = 0; j < (int)sizeof(T) / 2; j++) w[j] = reinterpret_cast<const uint4 *>(t)[j];
+    }
   }
+};
+// The largest magnitude by its bits, whose integer order keeps a NaN above
+// everything; 16-bit types two at a time until the end.
+template <typename T> __device__ __forceinline__ uint32_t join_bits(uint32_t a, uint32_t b) {
+  return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b);
 }
-__device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
+template <typename T> __device__ __forceinline__ uint32_t largest_bits(const Eight<T> &e) {
+  constexpr uint32_t MASK = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
   uint32_t b = 0;
 #pragma unroll
-  for (int j = 0; j < 8; j++) b = max(b, __float_as_uint(v[j]) & 0x7fffffffu);
+  for (int j = 0; j < (int)sizeof(T) / 2; j++)
+    b = join_bits<T>(b, join_bits<T>(join_bits<T>(e.w[j].x & MASK, e.w[j].y & MASK),
+                                     join_bits<T>(e.w[j].z & MASK, e.w[j].w & MASK)));
   return b;
 }
-// The codes of 8 values, rounded to nearest (ties to even) by the hardware's conversion.
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inverse) {
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++)
-    w[j] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(v[2 * j], inverse), __fmul_rn(v[2 * j + 1], inverse)),
-                                    __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+// The bits of the FP32 value of that magnitude.
+__device__ __forceinline__ uint32_t float_bits(uint32_t b, const float *) { return b; }
+__device__ __forceinline__ uint32_t float_bits(uint32_t b, const __half *) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(b & 0xffffu, b >> 16))));
+}
+__device__ __forceinline__ uint32_t float_bits(uint32_t b, const __nv_bfloat16 *) { return max(b & 0xffffu, b >> 16) << 16; }
+
+__device__ __forceinline__ float2 two_floats(uint32_t w, const __half *) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ float2 two_floats(uint32_t w, const __nv_bfloat16 *) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// The codes of two values, rounded to nearest (ties to even) by the hardware's conversion.
+__device__ __forceinline__ uint32_t codes2(float2 v, float inverse) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(v.x, inverse), __fmul_rn(v.y, inverse)), __NV_SATFINITE,
+                                  __NV_E4M3);
+}
+__device__ __forceinline__ uint2 codes8(const Eight<float> &e, float inverse) {
+  auto four = [&](const uint4 &w) {
+    return codes2(make_float2(__uint_as_float(w.x), __uint_as_float(w.y)), inverse) |
+           (codes2(make_float2(__uint_as_float(w.z), __uint_as_float(w.w)), inverse) << 16);
+  };
+  return make_uint2(four(e.w[0]), four(e.w[1]));
+}
+template <typename T> __device__ __forceinline__ uint2 codes8(const Eight<T> &e, float inverse) {
+  auto four = [&](uint32_t a, uint32_t b) {
+    return codes2(two_floats(a, static_cast<T *>(nullptr)), inverse) |
+           (codes2(two_floats(b, static_cast<T *>(nullptr)), inverse) << 16);
+  };
+  return make_uint2(four(e.w[0].x, e.w[0].y), four(e.w[0].z, e.w[0].w));
 }
 
 // Blocks of 1 x 128: 16 lanes a block, 8 values a lane, read once and kept in
-// registers. Bound by memory: UNITS blocks a half warp are in flight.
+// registers; a warp 8 blocks, their loads all in flight. Bound by memory if the
+// instructions are few: lane l of a half works out the scale of the half's
+// block l % 4, so the two divisions are done once for the 8. (1,000,000 x 768
+// FP16: see the table in the design notes.)
 constexpr int kQuantUnits = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows(const T *x, uint64_t stride, uint64_t blocks, uint32_t k,
-                                                     uint32_t kb, uint8_t *codes, uint64_t code_stride,
-                                                     float *scales) {
-  const uint32_t lane = threadIdx.x & 15;
+                                                     uint32_t kb, uint32_t rows2, uint32_t blocks2, uint8_t *codes,
+                                                     uint64_t code_stride, float *scales) {
+  const uint32_t lane = threadIdx.x & 15, half = (threadIdx.x >> 4) & 1;
   const bool vec = stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const uint32_t k16 = (k + 15) / 16 * 16;
-  const uint64_t u0 = ((uint64_t)blockIdx.x * 16 + threadIdx.x / 16) * kQuantUnits;
-  float v[kQuantUnits][8];
-  uint64_t row[kQuantUnits];
+  // this half's blocks: u0, u0 + 2, u0 + 4, u0 + 6
+  const uint64_t u0 = ((uint64_t)blockIdx.x * 8 + threadIdx.x / 32) * (2 * kQuantUnits) + half;
+  Eight<T> e[kQuantUnits];
   uint32_t col[kQuantUnits];
-  row[0] = blocks < 0x80000000ull ? (uint32_t)u0 / kb : u0 / kb;
-  uint32_t b = (uint32_t)(u0 - row[0] * kb);
+  uint64_t row = blocks < 0x80000000ull ? (uint32_t)u0 / kb : u0 / kb;
+  uint32_t b = (uint32_t)(u0 - row * kb);
+  uint8_t *to[kQuantUnits];
 #pragma unroll
   for (int u = 0; u < kQuantUnits; u++) {
-    if (u > 0) row[u] = row[u - 1];
-    if (b == kb) {
-      b = 0;
-      row[u]++;
+    col[u] = b * kBlock + lane * 8;
+    to[u] = codes + row * code_stride + col[u];
+    if (u0 + 2 * u < blocks) e[u].load(x + row * stride, col[u], k, vec);
+    // two blocks on: rows2 whole rows and blocks2 blocks
+    row += rows2;
+    b += blocks2;
+    if (b >= kb) {
+      b -= kb;
+      row++;
     }
-    col[u] = b++ * kBlock + lane * 8;
-    if (u0 + u < blocks) load8(x + row[u] * stride, col[u], k, vec, v[u]);
   }
+  uint32_t bits[kQuantUnits];
 #pragma unroll
   for (int u = 0; u < kQuantUnits; u++) {
-    const bool in = u0 + u < blocks;
-    uint32_t bits = in ? largest_bits(v[u]) : 0;
+    bits[u] = u0 + 2 * u < blocks ? largest_bits(e[u]) : 0;
 #pragma unroll
-    for (int d = 8; d; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
-    float inverse;
-    const float scale = block_scale(bits, inverse);
-    if (!in) continue;
-    if (lane == 0) scales[u0 + u] = scale;
-    if (col[u] < k16) *reinterpret_cast<uint2 *>(codes + row[u] * code_stride + col[u]) = codes8(v[u], inverse);
+    for (int d = 8; d; d >>= 1) bits[u] = join_bits<T>(bits[u], __shfl_xor_sync(0xffffffffu, bits[u], d));
+  }
+  const uint32_t mine = (lane & 2) ? ((lane & 1) ? bits[3] : bits[2]) : ((lane & 1) ? bits[1] : bits[0]);
+  float inverse;
+  const float scale = block_scale(float_bits(mine, static_cast<T *>(nullptr)), inverse);
+  if (lane < kQuantUnits && u0 + 2 * lane < blocks) scales[u0 + 2 * lane] = scale;
+#pragma unroll
+  for (int u = 0; u < kQuantUnits; u++) {
+    const float inv = __shfl_sync(0xffffffffu, inverse, u, 16);
+    if (u0 + 2 * u < blocks && col[u] < k16) *reinterpret_cast<uint2 *>(to[u]) = codes8(e[u], inv);
   }
 }
 
@@ -109,17 +152,16 @@ __global__ void __launch_bounds__(256) quantize_square(const T *x, uint64_t stri
   const uint32_t k16 = (k + 15) / 16 * 16;
   const uint64_t r0 = (uint64_t)(blockIdx.x / kb) * kBlock + threadIdx.x / 16;
   const uint32_t c = blockIdx.x % kb * kBlock + lane * 8;
-  float v[8][8];
+  Eight<T> e[8];
+#pragma unroll
+  for (int u = 0; u < 8; u++)
+    if (r0 + 16 * u < m) e[u].load(x + (r0 + 16 * u) * stride, c, k, vec);
   uint32_t bits = 0;
 #pragma unroll
-  for (int u = 0; u < 8; u++) {
-    if (r0 + 16 * u < m) {
-      load8(x + (r0 + 16 * u) * stride, c, k, vec, v[u]);
-      bits = max(bits, largest_bits(v[u]));
-    }
-  }
+  for (int u = 0; u < 8; u++)
+    if (r0 + 16 * u < m) bits = join_bits<T>(bits, largest_bits(e[u]));
   __shared__ uint32_t top[8];
-  bits = __reduce_max_sync(0xffffffffu, bits);
+  bits = __reduce_max_sync(0xffffffffu, float_bits(bits, static_cast<T *>(nullptr)));
   if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = bits;
   __syncthreads();
   bits = 0;
@@ -131,8 +173,7 @@ __global__ void __launch_bounds__(256) quantize_square(const T *x, uint64_t stri
   if (c >= k16) return;
 #pragma unroll
   for (int u = 0; u < 8; u++)
-    if (r0 + 16 * u < m)
-      *reinterpret_cast<uint2 *>(codes + (r0 + 16 * u) * code_stride + c) = codes8(v[u], inverse);
+    if (r0 + 16 * u < m) *reinterpret_cast<uint2 *>(codes + (r0 + 16 * u) * code_stride + c) = codes8(e[u], inverse);
 }
 
 template <typename T>
@@ -145,7 +186,7 @@ void launch_quantize(const T *x, uint64_t stride, uint64_t m, uint32_t k, bool s
   } else {
     const uint64_t blocks = m * kb;
     quantize_rows<<<(unsigned)((blocks + 16 * kQuantUnits - 1) / (16 * kQuantUnits)), 256, 0, st>>>(
-        x, stride, blocks, k, kb, codes, code_stride, scales);
+        x, stride, blocks, k, kb, 2 / kb, 2 % kb, codes, code_stride, scales);
   }
 }
 
