@@ -2,9 +2,9 @@
 // product of two operands in that form (AnnB200QuantizeBlocks,
 // AnnB200MatmulBlocks).
 //
-// The product has two kernels. With up to 4 rows in a (single queries) it is
-// bound by reading b once: a warp a few rows of b, CUDA cores. Above that the
-// tensor cores (pair_gemm.cuh): a K block of 128 is one sum in tensor memory,
+// The product has two kernels. With up to 8 rows in a (single queries) it is
+// bound by reading b once: a warp 16 rows of b, straight into registers. Above
+// that the pairs of SMs of pair_gemm.cuh: a K block of 128 is one sum in tensor memory,
 // which the epilogue takes out, scales and adds up in FP32 registers while the
 // next block's products run.
 #include <cuda_fp8.h>
@@ -202,15 +202,6 @@ struct Operands {
   uint64_t out_stride;
 };
 
-// Four E4M3 codes -> two pairs of FP32 (through FP16, which holds them all).
-__device__ __forceinline__ void decode4(uint32_t w, f32x2 &lo, f32x2 &hi) {
-  const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-  const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-  const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a));
-  const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
-  lo = pack2(x.x, x.y);
-  hi = pack2(y.x, y.y);
-}
 // 16 codes of a row from column c on; those past k are zero.
 __device__ __forceinline__ uint4 load16(const uint8_t *row, uint32_t c, uint32_t k) {
   if (c >= k) return make_uint4(0, 0, 0, 0);
@@ -225,69 +216,78 @@ __device__ __forceinline__ uint4 load16(const uint8_t *row, uint32_t c, uint32_t
   }
   return w;
 }
+// 16 x 8 sums of 32 codes each: the warp-level instruction, whose operands come
+// straight from registers (bound by reading b, nothing is gained by staging).
+__device__ __forceinline__ void mma_16x8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
-// A warp kFewRows rows of b against all M rows of a: 16 codes a lane, 512 of K
-// a step (8 lanes a block), each lane's products times its block's scales into
-// its own FP32 sums; the lanes' sums joined at the end.
-constexpr int kFewRows = 4;
-template <int M, typename T>
-__global__ void __launch_bounds__(256, M == 1 ? 3 : 2) matmul_few(const Operands p, T *out) {
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t n0 = ((uint64_t)blockIdx.x * 8 + warp) * kFewRows;
-  if (n0 >= p.n) return;
-  float sum[kFewRows][M] = {};
-  const uint8_t *brow[kFewRows];
-  const float *bscale[kFewRows];
-#pragma unroll
-  for (int r = 0; r < kFewRows; r++) {
-    const uint64_t n = min(n0 + r, p.n - 1);
-    brow[r] = p.b + n * p.b_stride;
-    bscale[r] = p.b_scales + (n >> p.b_shift) * p.kb;
+// Up to 8 rows in a: a warp 16 rows of b against all of them, a block of 128 at
+// a time. A thread (row l / 4, quarter l % 4) reads 32 codes of rows l / 4 and
+// + 8 of b and of row l / 4 of a; which of the 128 a register stands for does
+// not matter as long as both operands agree. The block's sums are scaled and
+// added up in FP32. SPLIT warps share 16 rows, each every SPLIT-th block, and
+// join their sums in shared memory: for few rows of b.
+constexpr int kFewWarps = 8;
+template <int SPLIT, typename T>
+__global__ void __launch_bounds__(32 * kFewWarps) matmul_few(const Operands p, T *out) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+  const uint32_t part = warp % SPLIT;
+  const uint64_t n0 = ((uint64_t)blockIdx.x * (kFewWarps / SPLIT) + warp / SPLIT) * 16;
+  // rows past the ends read the last one's codes; their results are not stored
+  const uint64_t na = min(n0 + r, p.n - 1), nb = min(n0 + r + 8, p.n - 1), m = min((uint64_t)r, p.m - 1);
+  const uint8_t *ba = p.b + na * p.b_stride, *bb = p.b + nb * p.b_stride, *a = p.a + m * p.a_stride;
+  const float *sba = p.b_scales + (na >> p.b_shift) * p.kb, *sbb = p.b_scales + (nb >> p.b_shift) * p.kb;
+  const float *sa0 = p.a_scales + (min((uint64_t)(2 * q), p.m - 1) >> p.a_shift) * p.kb;
+  const float *sa1 = p.a_scales + (min((uint64_t)(2 * q + 1), p.m - 1) >> p.a_shift) * p.kb;
+  float sum[4] = {};
+#pragma unroll 4
+  for (uint32_t b = part; b < p.kb; b += SPLIT) {
+    const uint32_t c = b * kBlock + q * 32;
+    const uint4 xa = load16(ba, c, p.k), ya = load16(ba, c + 16, p.k), xb = load16(bb, c, p.k),
+                yb = load16(bb, c + 16, p.k), xm = load16(a, c, p.k), ym = load16(a, c + 16, p.k);
+    const float s0 = __ldg(sa0 + b), s1 = __ldg(sa1 + b), ra = __ldg(sba + b), rb = __ldg(sbb + b);
+    float d[4] = {};
+    mma_16x8(d, xa.x, xb.x, xa.y, xb.y, xm.x, xm.y);
+    mma_16x8(d, xa.z, xb.z, xa.w, xb.w, xm.z, xm.w);
+    mma_16x8(d, ya.x, yb.x, ya.y, yb.y, ym.x, ym.y);
+    mma_16x8(d, ya.z, yb.z, ya.w, yb.w, ym.z, ym.w);
+    sum[0] = fmaf(d[0], ra * s0, sum[0]);
+    sum[1] = fmaf(d[1], ra * s1, sum[1]);
+    sum[2] = fmaf(d[2], rb * s0, sum[2]);
+    sum[3] = fmaf(d[3], rb * s1, sum[3]);
   }
-#pragma unroll 2
-  for (uint32_t c = lane * 16; c < p.k; c += 512) {
-    uint4 wb[kFewRows];
-    float sb[kFewRows];
-#pragma unroll
-    for (int r = 0; r < kFewRows; r++) {
-      wb[r] = load16(brow[r], c, p.k);
-      sb[r] = __ldg(bscale[r] + c / kBlock);
-    }
-#pragma unroll
-    for (int i = 0; i < M; i++) {
-      const uint64_t m = i < p.m ? i : p.m - 1;
-      const uint4 wa = load16(p.a + m * p.a_stride, c, p.k);
-      const float sa = __ldg(p.a_scales + (m >> p.a_shift) * p.kb + c / kBlock);
-      f32x2 av[8];
-      decode4(wa.x, av[0], av[1]);
-      decode4(wa.y, av[2], av[3]);
-      decode4(wa.z, av[4], av[5]);
-      decode4(wa.w, av[6], av[7]);
-#pragma unroll
-      for (int r = 0; r < kFewRows; r++) {
-        f32x2 bv[8];
-        decode4(wb[r].x, bv[0], bv[1]);
-        decode4(wb[r].y, bv[2], bv[3]);
-        decode4(wb[r].z, bv[4], bv[5]);
-        decode4(wb[r].w, bv[6], bv[7]);
-        f32x2 d[2] = {mul2(av[0], bv[0]), mul2(av[1], bv[1])};
-#pragma unroll
-        for (int j = 2; j < 8; j++) d[j & 1] = fma2(av[j], bv[j], d[j & 1]);
-        float x, y;
-        unpack2(add2(d[0], d[1]), x, y);
-        sum[r][i] = fmaf(x + y, sa * sb[r], sum[r][i]);
-      }
+  if (SPLIT > 1) {
+    __shared__ float4 joined[kFewWarps][32];
+    joined[warp][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    if (part != 0) return;
+    for (int w = 1; w < SPLIT; w++) {
+      const float4 v = joined[warp + w][lane];
+      sum[0] += v.x;
+      sum[1] += v.y;
+      sum[2] += v.z;
+      sum[3] += v.w;
     }
   }
 #pragma unroll
-  for (int r = 0; r < kFewRows; r++)
-#pragma unroll
-    for (int i = 0; i < M; i++) {
-      float s = sum[r][i];
-#pragma unroll
-      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      if (lane == 0 && n0 + r < p.n && i < p.m) out[(uint64_t)i * p.out_stride + n0 + r] = from_float<T>(s);
-    }
+  for (int j = 0; j < 4; j++) {
+    const uint64_t n = n0 + r + 8 * (j >> 1);
+    const uint32_t i = 2 * q + (j & 1);
+    if (n < p.n && i < p.m) out[(uint64_t)i * p.out_stride + n] = from_float<T>(sum[j]);
+  }
+}
+
+template <int SPLIT, typename T>
+cudaError_t launch_few(const Operands &o, T *out, cudaStream_t st) {
+  const uint64_t rows = 16 * (kFewWarps / SPLIT);
+  matmul_few<SPLIT><<<(unsigned)((o.n + rows - 1) / rows), 32 * kFewWarps, 0, st>>>(o, out);
+  return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------- product, tensor cores
@@ -359,7 +359,8 @@ struct ScaleStage {
     return true;
   }
   // The epilogue's: shared address of block b's scales, and the end of its use.
-  __device__ __forceinline__ uint32_t take(uint32_t b, PairSums &sums) const {
+  template <typename Sums>
+  __device__ __forceinline__ uint32_t take(uint32_t b, Sums &sums) const {
     if (b % AHEAD == 0 && sums.ok)
       sums.ok = __all_sync(0xffffffffu, pair_wait(bars() + (group & 1), (group >> 1) & 1, sums.abort));
     return smem_u32(scratch) + (group & 1) * BUFFER + (b % AHEAD) * (ROW * 4);
@@ -401,6 +402,8 @@ struct NarrowOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  // a block's sum passes from role to role in about 1,000 clocks, in which b's next blocks arrive
+  static constexpr int ACCS = 2 * COLS >= 128 ? 4 : 8;
   using Scales = ScaleStage<128, 2 * COLS>;
   static constexpr int SCRATCH = Scales::BYTES;
   using Args = BlocksArgs<T>;
@@ -426,7 +429,7 @@ struct NarrowOp {
         return;
     }
   }
-  static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
+  static __device__ __forceinline__ void epilogue(const Args &p, PairSumsOf<ACCS> &sums, uint8_t *scratch, uint32_t rank,
                                                   uint32_t cluster, uint32_t clusters) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, quad = warp & 3;
     const Operands &o = p.o;
@@ -505,7 +508,7 @@ template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
+  static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2, ACCS = 2;
   using Scales = ScaleStage<128, UNIFORM ? 2 : 256, std::conditional_t<UNIFORM, InOrder, PatchOrder>>;
   static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024;
   static constexpr int SCRATCH = SCALE_BYTES + kPairEpi * kBoxBytes;
@@ -700,17 +703,19 @@ cudaError_t launch_tiles(const Operands &o, T *out, bool wide, uint32_t bn, int 
 
 template <typename T>
 cudaError_t launch_matmul(const Operands &o, T *out, cudaStream_t st) {
-  if (o.m <= 4) {
-    const unsigned grid = (unsigned)((o.n + 8 * kFewRows - 1) / (8 * kFewRows));
-    if (o.m == 1) matmul_few<1><<<grid, 256, 0, st>>>(o, out);
-    else if (o.m == 2) matmul_few<2><<<grid, 256, 0, st>>>(o, out);
-    else matmul_few<4><<<grid, 256, 0, st>>>(o, out);
-    return cudaGetLastError();
+  if (o.m <= 8) {
+    // enough warps for every SM, as long as each has blocks of its own
+    const uint64_t warps = (o.n + 15) / 16, want = 148 * 16;
+    if (warps >= want || o.kb < 2) return launch_few<1>(o, out, st);
+    if (warps * 2 >= want || o.kb < 4) return launch_few<2>(o, out, st);
+    if (warps * 4 >= want || o.kb < 8) return launch_few<4>(o, out, st);
+    return launch_few<8>(o, out, st);
   }
   const int sms = op_sms();
   if (sms < 2) return cudaErrorNoDevice;
   // columns a thread: the fewest that hold a's rows in one tile
   if (o.m <= 32) return launch_tiles<NarrowOp<16, T>>(o, out, false, 32, sms, st);
+  if (o.m <= 64) return launch_tiles<NarrowOp<32, T>>(o, out, false, 64, sms, st);
   if (o.m <= 128) return launch_tiles<NarrowOp<64, T>>(o, out, false, 128, sms, st);
   return o.b_shift ? launch_tiles<WideOp<true, T>>(o, out, true, 256, sms, st)
                    : launch_tiles<WideOp<false, T>>(o, out, true, 256, sms, st);

@@ -16,8 +16,8 @@
 //              publishes the sums in both CTAs.
 //   10 and 11  an operator's helpers, if it has any.
 //
-// Two sums of 256 columns each let the epilogue of one run under the products
-// of the next. The tensor cores cut off, and do not round, what falls below a
+// Two sums of 256 columns each (more, where a tile has fewer columns) let the
+// epilogue of one run under the products of the next. The tensor cores cut off, and do not round, what falls below a
 // sum's last bit: over 48 steps of 16 (768 dimensions) that came to 1.4e-6 of
 // the sum, all of one sign, against 3e-8 in FP32 arithmetic. So an operator
 // whose result keeps 24 bits takes a sum over CHUNK K blocks and adds the
@@ -204,7 +204,9 @@ struct BoxStore {
 
 // What an epilogue warp needs of the loop: the sums of one accumulator after
 // another. `ok` stays false once a wait has run out.
-struct PairSums {
+template <int ACCS>
+struct PairSumsOf {
+  static constexpr uint32_t WIDTH = 512 / ACCS;   // columns of an accumulator
   uint64_t *full;
   uint32_t empty_leader;     // cluster address of the leader's empty[0]
   volatile uint32_t *abort;
@@ -213,14 +215,14 @@ struct PairSums {
   bool ok;
   // Tensor memory address of the next accumulator's columns for this warp's lanes.
   __device__ __forceinline__ uint32_t acquire() {
-    if (ok) ok = __all_sync(0xffffffffu, pair_wait(full + (n & 1), (n >> 1) & 1, abort));
+    if (ok) ok = __all_sync(0xffffffffu, pair_wait(full + n % ACCS, (n / ACCS) & 1, abort));
     tc_fence_after();
-    return tmem + (n & 1) * 256;
+    return tmem + (n % ACCS) * WIDTH;
   }
   __device__ __forceinline__ void release() {
     tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0 && ok) remote_arrive(empty_leader + (n & 1) * 8);
+    if ((threadIdx.x & 31) == 0 && ok) remote_arrive(empty_leader + (n % ACCS) * 8);
     n++;
   }
   // N x 32 columns from `at` on, of the item's whole K: its chunks, added up.
@@ -270,12 +272,14 @@ struct PairSums {
   }
 };
 
+using PairSums = PairSumsOf<2>;
+
 // The shared memory of an operator's loop: stages of (A planes, B planes), the
 // epilogue's scratch, barriers.
 template <class Op>
 struct PairShape {
   static constexpr int A_BYTES = Op::PLANES * kPairTileBytes;
-  static constexpr int BAR_BYTES = 256;
+  static constexpr int BAR_BYTES = 384;
   // b_bytes: one plane's B tile of this CTA
   static __host__ __device__ constexpr int stage(int b_bytes) { return A_BYTES + Op::PLANES * b_bytes; }
   static __host__ __device__ constexpr int stages(int b_bytes) {
@@ -286,12 +290,13 @@ struct PairShape {
 };
 
 // Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
-// sum; 0: the item's), HELPERS (0 or 2 warps), Args with maps a[PLANES],
+// sum; 0: the item's), ACCS (sums in tensor memory at a time: 512 / ACCS >= bn),
+// HELPERS (0 or 2 warps), Args with maps a[PLANES],
 // b[PLANES] and bn (columns of a tile), items(args), item(args, i),
 // epilogue(args, sums, scratch, rank, cluster, clusters): all of the cluster's
 // items; init and help where there are helpers.
 struct PairNoHelpers {
-  static constexpr int HELPERS = 0;
+  static constexpr int HELPERS = 0, ACCS = 2;
   static __device__ __forceinline__ void init(uint8_t *) {}
   template <class Args>
   static __device__ __forceinline__ void help(const Args &, uint8_t *, uint32_t, uint32_t, uint32_t,
@@ -304,7 +309,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   using Shape = PairShape<Op>;
   constexpr int PLANES = Op::PLANES;
   constexpr int KE = Op::KIND == PAIR_E4M3 ? 128 : 64;   // K elements of a block
-  constexpr int MAXS = Op::MAX_STAGES;
+  constexpr int MAXS = Op::MAX_STAGES, ACCS = Op::ACCS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t b_bytes = args.bn * 64;                 // bn / 2 rows (or columns) of 128 bytes each K block
@@ -314,11 +319,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t *full = reinterpret_cast<uint64_t *>(scratch + Op::SCRATCH);
   uint64_t *empty = full + MAXS;
   uint64_t *tfull = empty + MAXS;
-  uint64_t *tempty = tfull + 2;
-  uint64_t *drain = tempty + 2;
+  uint64_t *tempty = tfull + ACCS;
+  uint64_t *drain = tempty + ACCS;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile uint32_t *abort = tmem_slot + 1;
-  static_assert((2 * MAXS + 5) * 8 + 8 <= Shape::BAR_BYTES, "barriers");
+  static_assert((2 * MAXS + 2 * ACCS + 1) * 8 + 8 <= Shape::BAR_BYTES, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
@@ -330,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       mbar_init(full + s, 1);
       mbar_init(empty + s, 1);
     }
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < ACCS; b++) {
       mbar_init(tfull + b, 1);
       mbar_init(tempty + b, 2 * kPairEpi);
     }
@@ -352,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   if (warp < kPairEpi) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpiRegs));
-    PairSums sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
+    PairSumsOf<ACCS> sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
     Op::epilogue(args, sums, scratch, rank, cluster, clusters);
     BoxStore::finish();
   } else {
@@ -407,7 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           for (uint32_t kb = 0; kb < w.kblocks; kb++) {
             const bool first = Op::CHUNK ? kb % (Op::CHUNK + !Op::CHUNK) == 0 : kb == 0;
             const bool last = kb + 1 == w.kblocks || (Op::CHUNK && (kb + 1) % (Op::CHUNK + !Op::CHUNK) == 0);
-            if (first && !pair_wait(tempty + (acc & 1), ((acc >> 1) & 1) ^ 1, abort)) {
+            if (first && !pair_wait(tempty + acc % ACCS, ((acc / ACCS) & 1) ^ 1, abort)) {
               ok = false;
               break;
             }
@@ -416,7 +421,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               break;
             }
             tc_fence_after();
-            const uint32_t d = tmem + (acc & 1) * 256;
+            const uint32_t d = tmem + (acc % ACCS) * (512 / ACCS);
             const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + Shape::A_BYTES;
             auto adesc = [&](uint32_t p, uint32_t kk) {
               const uint32_t at = a + p * kPairTileBytes + kk * A_STEP;
@@ -436,7 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             pair_commit(empty + s);
             if (last) {
-              pair_commit(tfull + (acc & 1));
+              pair_commit(tfull + acc % ACCS);
               acc++;
             }
             if (++s == stages) {
