@@ -32,8 +32,6 @@ constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial ma
 constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece, where a piece has 8,192 rows by then
 constexpr uint32_t kPlanClusters = 74;          // clusters the plan splits for (148 SMs)
 
-enum { MAX_ROWS = 0, MAX_QUERIES = 1, MAX_GRAD = 2 };   // the workspace's maxima (float bits)
-
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -55,102 +53,164 @@ __device__ __forceinline__ bool has_target(int64_t t, uint64_t nrows) { return t
 
 // ---------------------------------------------------------------- laying operands out
 
-// The largest finite |x| of an FP32 array (bits, by atomicMax: any order gives
-// the same). Threads cover `tx` 4-value chunks of a row and 256 / tx rows.
-__global__ void __launch_bounds__(256) array_max(const float *x, uint64_t stride, uint64_t rows, uint32_t dims,
-                                                 uint32_t tx, const int64_t *targets, uint64_t nrows, uint32_t *out) {
-  const uint32_t cx = threadIdx.x % tx, ry = threadIdx.x / tx, ty = 256 / tx;
-  const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+// Maxima are found in two steps without atomics or a cleared word: a grid leaves
+// one a block, and whoever needs the whole array's joins them.
+constexpr int kRowParts = 592, kQueryParts = 64, kGradParts = 32;
+struct Maxima {
+  uint32_t rows[kRowParts], queries[kQueryParts], grad[kGradParts];
+  uint32_t all_rows, all_queries;   // joined by the layout kernel
+};
+// The largest of n <= 1024 parts, for every thread of a 256-thread block.
+__device__ __forceinline__ uint32_t block_max(uint32_t best) {
+  __shared__ uint32_t top[8];
+  best = __reduce_max_sync(0xffffffffu, best);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = best;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; i++) best = max(best, top[i]);
+  return best;
+}
+__device__ __forceinline__ uint32_t join_parts(const uint32_t *parts, int n) {
   uint32_t best = 0;
-  auto take = [&](float v) {
-    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-    if (b < 0x7f800000u) best = max(best, b);
-  };
-  for (uint64_t r = (uint64_t)blockIdx.x * ty + ry; r < rows; r += (uint64_t)gridDim.x * ty) {
-    if (targets && !has_target(targets[r], nrows)) continue;
-    const float *row = x + r * stride;
+  for (int i = threadIdx.x; i < n; i += 256) best = max(best, parts[i]);
+  return block_max(best);
+}
+// The gradient's unit (a warp's lanes together).
+__device__ __forceinline__ float grad_unit(const Maxima *m) {
+  static_assert(kGradParts == 32, "a part a lane");
+  return grad_unit(__reduce_max_sync(0xffffffffu, m->grad[threadIdx.x & 31]));
+}
+// A value's bits, 0 where it is not finite.
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// FP32: the largest finite |x| of the rows and, in the gradient, of the queries
+// with a target. `tx` threads a row, 4 values each.
+__global__ void __launch_bounds__(256) find_maxima(const float *w, uint64_t w_stride, uint64_t nrows, const float *x,
+                                                   uint64_t x_stride, uint32_t nq, uint32_t dims, uint32_t tx,
+                                                   const int64_t *targets, Maxima *out) {
+  const bool queries = blockIdx.x >= kRowParts;
+  const uint32_t block = queries ? blockIdx.x - kRowParts : blockIdx.x, grid = queries ? kQueryParts : kRowParts;
+  const float *from = queries ? x : w;
+  const uint64_t stride = queries ? x_stride : w_stride, rows = queries ? nq : nrows;
+  const uint32_t cx = threadIdx.x % tx, ry = threadIdx.x / tx, ty = 256 / tx;
+  const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+  uint32_t best = 0;
+  for (uint64_t r = (uint64_t)block * ty + ry; r < rows; r += (uint64_t)grid * ty) {
+    if (queries && !has_target(targets[r], nrows)) continue;
+    const float *row = from + r * stride;
     for (uint32_t c = cx * 4; c < dims; c += tx * 4) {
       if (vec && c + 4 <= dims) {
         const float4 v = __ldg(reinterpret_cast<const float4 *>(row + c));
-        take(v.x);
-        take(v.y);
-        take(v.z);
-        take(v.w);
+        best = max(max(best, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
       } else {
-        for (uint32_t j = c; j < min(dims, c + 4); j++) take(row[j]);
+        for (uint32_t j = c; j < min(dims, c + 4); j++) best = max(best, finite_bits(row[j]));
       }
     }
   }
-  best = __reduce_max_sync(0xffffffffu, best);
-  if (threadIdx.x % 32 == 0 && best) atomicMax(out, best);
+  best = block_max(best);
+  if (threadIdx.x == 0) (queries ? out->queries : out->rows)[block] = best;
 }
 
-// Per query 2^-e: of its own largest |x| (a warp a query), or the array's.
-__global__ void __launch_bounds__(256) query_scales(const float *x, uint64_t stride, uint32_t nq, uint32_t dims,
-                                                    const uint32_t *whole, float *scales) {
-  const uint32_t q = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x % 32;
-  if (q >= nq) return;
-  uint32_t best = whole ? *whole : 0;
-  if (!whole)
-    for (uint32_t c = lane; c < dims; c += 32) {
-      const uint32_t b = __float_as_uint(x[q * stride + c]) & 0x7fffffffu;
-      if (b < 0x7f800000u) best = max(best, b);
-    }
-  best = __reduce_max_sync(0xffffffffu, best);
-  if (lane == 0) scales[q] = undo_scale(best);
-}
-
-__global__ void __launch_bounds__(256) grad_max(const float *grad, const int64_t *targets, uint32_t nq, uint64_t nrows,
-                                                uint32_t *out) {
-  const uint32_t q = blockIdx.x * 256 + threadIdx.x;
-  uint32_t b = 0;
-  if (q < nq && has_target(targets[q], nrows)) b = grad ? __float_as_uint(grad[q]) & 0x7fffffffu : 0x3f800000u;
-  b = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
-  if (threadIdx.x % 32 == 0 && b) atomicMax(out, b);
-}
-
-// Rows of an operand in the layout TMA reads: `ld` values (a multiple of 8) a
-// row, values past dims zero. FP32: two FP16 planes of x * 2^e; an infinity
-// becomes NaN (its products with a low term of 0 would be). Queries without a
-// target (targets given) become rows of zeros.
+// Operands in the layout TMA reads: `ld` values (a multiple of 8) a row, values
+// past dims zero. FP32: two FP16 planes of x * 2^e; an infinity becomes NaN (its
+// products with a low term of 0 would be).
+template <typename T, typename O, int PLANES> struct Layout {
+  const T *x, *w;
+  uint64_t x_stride, w_stride, nrows;
+  uint32_t nq, dims, ld;
+  uint32_t tx;                     // threads a row of w, 8 values each
+  uint32_t query_blocks, row_blocks, grad_blocks;
+  const int64_t *targets;
+  const float *grad;
+  bool leave_out;                  // the gradient's: queries without a target become rows of zeros, one e for all
+  O *xo, *wo;
+  float *xscale;                   // PLANES 2: 2^-e of each query
+  Maxima *maxima;
+};
 template <typename T, typename O, int PLANES>
-__global__ void __launch_bounds__(256) pack_rows(const T *x, uint64_t stride, uint64_t rows, uint32_t dims, uint32_t ld,
-                                                 uint32_t tx, const int64_t *targets, uint64_t nrows,
-                                                 const float *row_scales, const uint32_t *whole, O *out,
-                                                 uint64_t plane) {
-  const uint32_t cx = threadIdx.x % tx, ry = threadIdx.x / tx, ty = 256 / tx;
-  const bool vec = stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  const float mul = PLANES == 2 && !row_scales ? 1.0f / undo_scale(*whole) : 1.0f;   // powers of two: exact
-  for (uint64_t r = (uint64_t)blockIdx.x * ty + ry; r < rows; r += (uint64_t)gridDim.x * ty) {
-    const bool zero = targets && !has_target(targets[r], nrows);
-    const float s = PLANES == 2 && row_scales ? 1.0f / row_scales[r] : mul;
-    const T *row = x + r * stride;
-    for (uint32_t c = cx * 8; c < ld; c += tx * 8) {
-      alignas(16) T v[8];
-      if (!zero && vec && c + 8 <= dims) {
+__device__ __forceinline__ void pack8(const T *row, uint32_t c, uint32_t dims, bool vec, bool zero, float mul, O *out,
+                                      uint64_t plane) {
+  alignas(16) T v[8];
+  if (!zero && vec && c + 8 <= dims) {
 #pragma unroll
-        for (int j = 0; j < (int)(8 * sizeof(T) / 16); j++)
-          reinterpret_cast<uint4 *>(v)[j] = __ldg(reinterpret_cast<const uint4 *>(row + c) + j);
-      } else {
+    for (int j = 0; j < (int)(8 * sizeof(T) / 16); j++)
+      reinterpret_cast<uint4 *>(v)[j] = __ldg(reinterpret_cast<const uint4 *>(row + c) + j);
+  } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = !zero && c + j < dims ? row[c + j] : from_float<T>(0.0f);
-      }
-      alignas(16) O hi[8], lo[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        if (PLANES == 2) {
-          float f = to_float(v[j]) * s;
-          if (isinf(f)) f = NAN;
-          hi[j] = from_float<O>(f);
-          lo[j] = from_float<O>(isnan(f) ? 0.0f : f - to_float(hi[j]));
-        } else {
-          reinterpret_cast<uint16_t *>(hi)[j] = reinterpret_cast<const uint16_t *>(v)[j];
-        }
-      }
-      *reinterpret_cast<uint4 *>(out + r * ld + c) = *reinterpret_cast<uint4 *>(hi);
-      if (PLANES == 2) *reinterpret_cast<uint4 *>(out + plane + r * ld + c) = *reinterpret_cast<uint4 *>(lo);
-    }
+    for (int j = 0; j < 8; j++) v[j] = !zero && c + j < dims ? row[c + j] : from_float<T>(0.0f);
   }
+  if (PLANES == 1) {
+    *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<uint4 *>(v);
+    return;
+  }
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    float f[2], l[2];
+    __half h[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      f[u] = to_float(v[2 * j + u]) * mul;
+      if (isinf(f[u])) f[u] = NAN;
+      h[u] = __float2half_rn(f[u]);
+      l[u] = isnan(f[u]) ? 0.0f : f[u] - __half2float(h[u]);
+    }
+    hi[j] = pack16<__half>(f[0], f[1]);
+    lo[j] = pack16<__half>(l[0], l[1]);
+  }
+  *reinterpret_cast<uint4 *>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  *reinterpret_cast<uint4 *>(out + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+template <typename T, typename O, int PLANES>
+__global__ void __launch_bounds__(256) lay_out(const Layout<T, O, PLANES> p) {
+  uint32_t block = blockIdx.x;
+  if (block < p.query_blocks) {   // a warp a query
+    const uint32_t lane = threadIdx.x % 32;
+    const bool vec = p.x_stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0;
+    uint32_t all = 0;
+    if (PLANES == 2 && p.leave_out) {
+      all = join_parts(p.maxima->queries, kQueryParts);
+      if (block == 0 && threadIdx.x == 0) p.maxima->all_queries = all;
+    }
+    const uint32_t q = block * 8 + threadIdx.x / 32;
+    if (q >= p.nq) return;
+    const T *row = p.x + q * p.x_stride;
+    if (PLANES == 2 && !p.leave_out) {
+      for (uint32_t c = lane; c < p.dims; c += 32) all = max(all, finite_bits(to_float(row[c])));
+      all = __reduce_max_sync(0xffffffffu, all);
+    }
+    const bool zero = p.leave_out && !has_target(p.targets[q], p.nrows);
+    const float undo = undo_scale(all), mul = 1.0f / undo;   // powers of two: exact
+    for (uint32_t c = lane * 8; c < p.ld; c += 256)
+      pack8<T, O, PLANES>(row, c, p.dims, vec, zero, mul, p.xo + (uint64_t)q * p.ld + c, (uint64_t)p.nq * p.ld);
+    if (PLANES == 2 && lane == 0) p.xscale[q] = undo;
+    return;
+  }
+  block -= p.query_blocks;
+  if (block < p.row_blocks) {
+    const uint32_t cx = threadIdx.x % p.tx, ry = threadIdx.x / p.tx, ty = 256 / p.tx;
+    const bool vec = p.w_stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15) == 0;
+    float mul = 1.0f;
+    if (PLANES == 2) {
+      const uint32_t all = join_parts(p.maxima->rows, kRowParts);
+      mul = 1.0f / undo_scale(all);
+      if (block == 0 && threadIdx.x == 0) p.maxima->all_rows = all;
+    }
+    for (uint64_t r = (uint64_t)block * ty + ry; r < p.nrows; r += (uint64_t)p.row_blocks * ty)
+      for (uint32_t c = cx * 8; c < p.ld; c += p.tx * 8)
+        pack8<T, O, PLANES>(p.w + r * p.w_stride, c, p.dims, vec, false, mul, p.wo + r * p.ld + c, p.nrows * p.ld);
+    return;
+  }
+  block -= p.row_blocks;
+  uint32_t best = 0;
+  for (uint32_t q = block * 256 + threadIdx.x; q < p.nq; q += p.grad_blocks * 256)
+    if (has_target(p.targets[q], p.nrows)) best = max(best, p.grad ? finite_bits(p.grad[q]) : 0x3f800000u);
+  best = block_max(best);
+  if (threadIdx.x == 0) p.maxima->grad[block] = best;
 }
 
 // ---------------------------------------------------------------- logits
@@ -178,7 +238,7 @@ template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
 struct LogitsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? kPairEpi * kBoxBytes : 0, MAX_STAGES = 8;
+  static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? 2 * kPairEpi * kBoxBytes : 0, MAX_STAGES = 8;
   static constexpr int CHUNK = PLANES == 2 ? 2 : 6;   // 24 steps of the tensor cores
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];
@@ -188,13 +248,14 @@ struct LogitsOp : PairNoHelpers {
     uint64_t nrows, first;   // rows; the first one of this piece
     double scale2;           // scale * log2(e)
     const float *xscale;     // PLANES 2: per query
-    const uint32_t *maxima;
+    const Maxima *maxima;
     const int64_t *targets;
     float2 *part;            // forward: [query - q0][2 nt]
     float *tlogit;           // [query]
     const float *lse, *grad;
     CUtensorMap g[PLANES];   // gradient: G of the piece
-    float *gsum;             // [query][2 nt]: the stored G summed over a half tile
+    float *gsum;             // [query][gsums]: the stored G summed over a half tile, of all pieces
+    uint32_t gsums;
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
@@ -225,9 +286,10 @@ struct LogitsOp : PairNoHelpers {
   static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
                                                   uint32_t cluster, uint32_t clusters) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
-    const double scale2 = PLANES == 2 ? p.scale2 * (double)undo_scale(p.maxima[MAX_ROWS]) : p.scale2;
-    const float unit = GRAD ? grad_unit(p.maxima[MAX_GRAD]) : 1.0f;
-    BoxStore box{scratch + warp * kBoxBytes};
+    const double scale2 = PLANES == 2 ? p.scale2 * (double)undo_scale(p.maxima->all_rows) : p.scale2;
+    const float unit = GRAD ? grad_unit(p.maxima) : 1.0f;
+    BoxStore box{scratch + 2 * warp * kBoxBytes};
+    uint32_t turn = 0;
     Row next = row_of(p, cluster, rank);
     for (uint32_t i = cluster; i < items(p); i += clusters) {
       const PairItem w = item(p, i);
@@ -340,7 +402,8 @@ struct LogitsOp : PairNoHelpers {
         for (int plane = 0; plane < PLANES; plane++) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            box.reuse();
+            box.box = scratch + (2 * warp + (turn++ & 1)) * kBoxBytes;   // two boxes in turn
+            box.reuse<1>();
 #pragma unroll
             for (int c = 0; c < 8; c++) {
               uint32_t o[4];
@@ -360,14 +423,14 @@ struct LogitsOp : PairNoHelpers {
         float a, b;
         unpack2(add2(sum[0], sum[1]), a, b);
         s = a + b;
-        if (valid) p.gsum[(uint64_t)q * (2 * p.nt) + 2 * w.index + half] = s;
+        if (valid) p.gsum[(uint64_t)q * p.gsums + (uint32_t)(p.first / 128) + 2 * w.index + half] = s;
       }
     }
   }
 };
 
 // Join a query's partial sums: lse = (m + log2 s) ln 2, loss = lse - target logit.
-__global__ void __launch_bounds__(128) join_parts(const float2 *part, uint32_t n, uint32_t q0, uint64_t nrows,
+__global__ void __launch_bounds__(128) join_sums(const float2 *part, uint32_t n, uint32_t q0, uint64_t nrows,
                                                   const int64_t *targets, const float *tlogit, float *loss, float *lse,
                                                   int32_t *status) {
   const uint32_t q = q0 + blockIdx.x;
@@ -478,7 +541,7 @@ struct RowsOp : PairNoHelpers {
     uint32_t mt, nt, kblocks;
     uint32_t rows, dims;     // rows of the piece
     double scale;
-    const uint32_t *maxima;
+    const Maxima *maxima;
     T *out;                  // the piece's first row
     int boxes;               // out's rows are 16-byte aligned: `map` stores them
     CUtensorMap map;
@@ -495,8 +558,8 @@ struct RowsOp : PairNoHelpers {
                                               uint32_t rank) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t i = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
-    double f = p.scale * (double)grad_unit(p.maxima[MAX_GRAD]) / kGradScale;
-    if (PLANES == 2) f *= (double)undo_scale(p.maxima[MAX_QUERIES]);
+    double f = p.scale * (double)grad_unit(p.maxima) / kGradScale;
+    if (PLANES == 2) f *= (double)undo_scale(p.maxima->all_queries);
     const float factor = (float)f;
     const uint32_t cols = p.bn / 2;
     f32x2 v[64];
@@ -545,16 +608,6 @@ struct RowsOp : PairNoHelpers {
   }
 };
 
-// A piece's sums of G into each query's (a warp a query).
-__global__ void __launch_bounds__(256) fold_sums(const float *gsum, uint32_t n, uint32_t nq, int add, double *total) {
-  const uint32_t q = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x % 32;
-  if (q >= nq) return;
-  double s = 0.0;
-  for (uint32_t i = lane; i < n; i += 32) s += gsum[(uint64_t)q * n + i];
-  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  if (lane == 0) total[q] = s + (add ? total[q] : 0.0);
-}
-
 // dX_i = scale * (the partial sums, in order, - (sum_j G_ij) w_target); zero for
 // a query without a target. G's exact rows sum to 0, the rounded ones do not,
 // and rows near each other (a cluster's) make sum_j G_ij w_j the small
@@ -564,26 +617,53 @@ __global__ void __launch_bounds__(256) fold_sums(const float *gsum, uint32_t n, 
 // G_ij (w_j - w_target), and errors are relative to the differences.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t splits, uint32_t nq, uint32_t dims,
-                                                    double scale, const uint32_t *maxima, const double *total,
-                                                    const T *rows, uint64_t stride, const int64_t *targets,
-                                                    uint64_t nrows, T *out) {
+                                                    double scale, const Maxima *maxima, const float *gsum,
+                                                    uint32_t gsums, const T *rows, uint64_t stride,
+                                                    const int64_t *targets, uint64_t nrows, T *out) {
   const uint32_t q = blockIdx.x, ld = (dims + 3) / 4 * 4;
   const uint64_t plane = (uint64_t)nq * ld;
-  const double f = scale * (double)grad_unit(maxima[MAX_GRAD]) / kGradScale;
-  const float factor = (float)f;
-  const float undo = PLANES == 2 ? undo_scale(maxima[MAX_ROWS]) : 1.0f;
   const int64_t t = targets[q];
-  const bool kept = has_target(t, nrows);
-  const float left = kept ? -(float)total[q] : 0.0f;
-  const T *row = rows + (kept ? (uint64_t)t * stride : 0);
-  for (uint32_t d = threadIdx.x; d < dims; d += blockDim.x) {
-    float v = 0.0f;
-    if (kept) {
-      const float *at = part + (uint64_t)q * ld + d;
-      for (uint32_t k = 0; k < splits; k++) v += at[k * plane];
-      v = fmaf(left, to_float(row[d]), v * undo) * factor;
+  T *to = out + (uint64_t)q * dims;
+  if (!has_target(t, nrows)) {
+    for (uint32_t d = threadIdx.x; d < dims; d += 256) to[d] = from_float<T>(0.0f);
+    return;
+  }
+  const float factor = (float)(scale * (double)grad_unit(maxima) / kGradScale);
+  const float undo = PLANES == 2 ? undo_scale(maxima->all_rows) : 1.0f;
+  const T *row = rows + (uint64_t)t * stride;
+  const float *at = part + (uint64_t)q * ld;
+  constexpr uint32_t EACH = 4;     // dimensions a thread: loaded before the sum of G is waited for
+  float v[EACH], r[EACH];
+  auto load = [&](uint32_t d0) {
+#pragma unroll
+    for (uint32_t u = 0; u < EACH; u++) {
+      const uint32_t d = d0 + threadIdx.x + 256 * u;
+      v[u] = 0.0f;
+      r[u] = 0.0f;
+      if (d < dims) {
+        r[u] = to_float(row[d]);
+        for (uint32_t k = 0; k < splits; k++) v[u] += at[k * plane + d];
+      }
     }
-    out[(uint64_t)q * dims + d] = from_float<T>(v);
+  };
+  load(0);
+  __shared__ double sum[8];
+  double s = 0.0;
+  for (uint32_t i = threadIdx.x; i < gsums; i += 256) s += gsum[(uint64_t)q * gsums + i];
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (threadIdx.x % 32 == 0) sum[threadIdx.x / 32] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) s += sum[i];
+  const float left = -(float)s;
+  for (uint32_t d0 = 0; d0 < dims; d0 += 256 * EACH) {
+    if (d0) load(d0);
+#pragma unroll
+    for (uint32_t u = 0; u < EACH; u++) {
+      const uint32_t d = d0 + threadIdx.x + 256 * u;
+      if (d < dims) to[d] = from_float<T>(fmaf(left, r[u], v[u] * undo) * factor);
+    }
   }
 }
 
@@ -609,7 +689,7 @@ struct Plan {
   int planes;
   uint32_t ld;             // values a packed row
   bool pack_x, pack_w;
-  uint64_t x, w, xscale, maxima, part, tlogit, g, gsum, gtotal, dq, total;
+  uint64_t x, w, xscale, maxima, part, tlogit, g, gsum, dq, total;
   uint32_t nt, chunk;      // forward: row tiles; queries a launch
   uint64_t piece;          // gradient: rows a piece
   uint32_t bn, dt, splits; // dimensions a tile, tiles, shares of a piece in dX
@@ -623,7 +703,7 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
   p.ld = (uint32_t)up(j.dims, 8);
   p.pack_x = grad || !in_place(j.queries, j.query_stride, j.dtype);
   p.pack_w = !in_place(j.rows, j.row_stride, j.dtype);
-  p.maxima = c.take(16);
+  p.maxima = c.take(sizeof(Maxima));
   p.xscale = c.take(nq * 4);
   if (p.pack_x) p.x = c.take(nq * p.ld * 2 * p.planes);
   if (p.pack_w) p.w = c.take(j.nrows * p.ld * 2 * p.planes);
@@ -638,8 +718,7 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
     p.piece = std::max<uint64_t>(8192, kPieceBytes / (2 * p.planes * nq) / 256 * 256);
     p.piece = std::min<uint64_t>({p.piece, up(j.nrows, 256), 1u << 20});
     p.g = c.take(nq * p.piece * 2 * p.planes);
-    p.gsum = c.take(nq * (p.piece / 128) * 4);
-    p.gtotal = c.take(nq * 8);
+    p.gsum = c.take(nq * 2 * p.nt * 4);
     // 128 dimensions a tile where 256 would leave over an eighth of them empty
     const uint64_t full = up(j.dims, 256), fine = up(j.dims, 128);
     p.bn = fine * 8 < full * 7 ? 128 : 256;
@@ -662,24 +741,6 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
   return p;
 }
 
-template <typename T, typename O, int PLANES>
-void pack(const T *x, uint64_t stride, uint64_t rows, uint32_t dims, uint32_t ld, const int64_t *targets,
-          uint64_t nrows, const float *scales, const uint32_t *whole, O *out, cudaStream_t st) {
-  uint32_t tx = 1;
-  while (tx < 256 && tx * 8 < ld) tx *= 2;
-  const uint64_t blocks = (rows + 256 / tx - 1) / (256 / tx);
-  pack_rows<T, O, PLANES><<<(unsigned)std::min<uint64_t>(blocks, 1u << 16), 256, 0, st>>>(
-      x, stride, rows, dims, ld, tx, targets, nrows, scales, whole, out, rows * ld);
-}
-
-void max_of(const float *x, uint64_t stride, uint64_t rows, uint32_t dims, const int64_t *targets, uint64_t nrows,
-            uint32_t *out, cudaStream_t st) {
-  uint32_t tx = 1;
-  while (tx < 256 && tx * 4 < dims) tx *= 2;
-  const uint64_t blocks = (rows + 256 / tx - 1) / (256 / tx);
-  array_max<<<(unsigned)std::min<uint64_t>(blocks, 1184), 256, 0, st>>>(x, stride, rows, dims, tx, targets, nrows, out);
-}
-
 // T: the operands' type; O: the products'.
 template <typename T, typename O, PairKind KIND, int PLANES>
 int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
@@ -687,44 +748,53 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   const int sms = op_sms();
   if (sms < 2) return report_error(OP_BACKEND_ERROR, "no current CUDA device");
   uint8_t *ws = static_cast<uint8_t *>(j.workspace);
-  uint32_t *maxima = reinterpret_cast<uint32_t *>(ws + p.maxima);
+  Maxima *maxima = reinterpret_cast<Maxima *>(ws + p.maxima);
   float *xscale = reinterpret_cast<float *>(ws + p.xscale);
   const T *x = static_cast<const T *>(j.queries), *w = static_cast<const T *>(j.rows);
-  const int64_t *kept = grad ? j.targets : nullptr;   // the gradient leaves out queries without a target
   unsigned long long launches = 0;
   cudaError_t e = cudaSuccess;
 
   // operands as the tensor maps read them
-  if (PLANES == 2 || grad) {
-    e = cudaMemsetAsync(maxima, 0, 16, st);
-    if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss: %s", cudaGetErrorString(e));
-  }
-  if (grad) {
-    grad_max<<<(j.nq + 255) / 256, 256, 0, st>>>(j.grad, j.targets, j.nq, j.nrows, maxima + MAX_GRAD);
-    launches++;
-  }
-  if (PLANES == 2) {
-    const float *xf = reinterpret_cast<const float *>(x);
-    max_of(reinterpret_cast<const float *>(w), j.row_stride, j.nrows, j.dims, nullptr, 0, maxima + MAX_ROWS, st);
-    if (grad) max_of(xf, j.query_stride, j.nq, j.dims, kept, j.nrows, maxima + MAX_QUERIES, st);
-    query_scales<<<(j.nq + 7) / 8, 256, 0, st>>>(xf, j.query_stride, j.nq, j.dims, grad ? maxima + MAX_QUERIES : nullptr,
-                                                 xscale);
-    launches += grad ? 3 : 2;
-  }
   const O *xo = reinterpret_cast<const O *>(x), *wo = reinterpret_cast<const O *>(w);
   uint64_t xld = j.query_stride, wld = j.row_stride;
+  Layout<T, O, PLANES> lay = {};
+  lay.x = x;
+  lay.w = w;
+  lay.x_stride = j.query_stride;
+  lay.w_stride = j.row_stride;
+  lay.nrows = j.nrows;
+  lay.nq = j.nq;
+  lay.dims = j.dims;
+  lay.ld = p.ld;
+  lay.tx = 1;
+  while (lay.tx < 256 && lay.tx * 8 < p.ld) lay.tx *= 2;
+  lay.targets = j.targets;
+  lay.grad = j.grad;
+  lay.leave_out = grad;
+  lay.xscale = xscale;
+  lay.maxima = maxima;
   if (p.pack_x) {
-    O *to = reinterpret_cast<O *>(ws + p.x);
-    pack<T, O, PLANES>(x, j.query_stride, j.nq, j.dims, p.ld, kept, j.nrows, xscale, nullptr, to, st);
-    xo = to;
+    lay.query_blocks = (j.nq + 7) / 8;
+    xo = lay.xo = reinterpret_cast<O *>(ws + p.x);
     xld = p.ld;
-    launches++;
   }
   if (p.pack_w) {
-    O *to = reinterpret_cast<O *>(ws + p.w);
-    pack<T, O, PLANES>(w, j.row_stride, j.nrows, j.dims, p.ld, nullptr, 0, nullptr, maxima + MAX_ROWS, to, st);
-    wo = to;
+    const uint64_t per = 256 / lay.tx;
+    lay.row_blocks = (uint32_t)std::min<uint64_t>((j.nrows + per - 1) / per, PLANES == 2 ? 4736 : 1u << 16);
+    wo = lay.wo = reinterpret_cast<O *>(ws + p.w);
     wld = p.ld;
+  }
+  if (grad) lay.grad_blocks = kGradParts;
+  if (PLANES == 2) {
+    uint32_t tx = 1;
+    while (tx < 256 && tx * 4 < j.dims) tx *= 2;
+    find_maxima<<<kRowParts + (grad ? kQueryParts : 0), 256, 0, st>>>(
+        reinterpret_cast<const float *>(w), j.row_stride, j.nrows, reinterpret_cast<const float *>(x), j.query_stride,
+        j.nq, j.dims, tx, j.targets, maxima);
+    launches++;
+  }
+  if (const uint32_t blocks = lay.query_blocks + lay.row_blocks + lay.grad_blocks) {
+    lay_out<T, O, PLANES><<<blocks, 256, 0, st>>>(lay);
     launches++;
   }
   bool maps = true;
@@ -762,7 +832,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       // (a launch covers whole tiles of queries, except at their end)
       e = launch_pair<Op>(l, l.mt * l.nt, sms, st);
       if (e != cudaSuccess) break;
-      join_parts<<<n, 128, 0, st>>>(l.part, 2 * p.nt, q0, j.nrows, j.targets, l.tlogit, j.loss, j.lse, j.status);
+      join_sums<<<n, 128, 0, st>>>(l.part, 2 * p.nt, q0, j.nrows, j.targets, l.tlogit, j.loss, j.lse, j.status);
       launches += 2;
     }
     if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss: %s", cudaGetErrorString(e));
@@ -782,7 +852,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   l.grad = j.grad;
   map(l.g, g, p.piece, j.nq, p.piece, gplane, 32);
   l.gsum = reinterpret_cast<float *>(ws + p.gsum);
-  double *gtotal = reinterpret_cast<double *>(ws + p.gtotal);
+  l.gsums = 2 * p.nt;
   for (uint64_t first = 0; first < j.nrows && e == cudaSuccess; first += p.piece) {
     const uint64_t n = std::min(p.piece, j.nrows - first);
     l.first = first;
@@ -802,9 +872,8 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       a.dims = j.dims;
       a.add = first != 0;
       maps = maps && encode_sums_map(&a.part, dq, j.dims, j.nq, p.splits, up(j.dims, 4) * 4);
-      fold_sums<<<(j.nq + 7) / 8, 256, 0, st>>>(l.gsum, 2 * l.nt, j.nq, a.add, gtotal);
       e = maps ? launch_pair<QOp>(a, a.mt * a.nt * a.splits, sms, st) : cudaErrorInvalidValue;
-      launches += 2;
+      launches++;
     }
     if (j.drows && e == cudaSuccess) {
       typename ROp::Args a = {};
@@ -829,9 +898,8 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   }
   if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss gradient: %s", cudaGetErrorString(e));
   if (j.dqueries) {
-    join_queries<T, PLANES><<<j.nq, j.dims <= 128 ? 128 : 256, 0, st>>>(
-        dq, p.splits, j.nq, j.dims, (double)j.scale, maxima, gtotal, w, j.row_stride, j.targets, j.nrows,
-        static_cast<T *>(j.dqueries));
+    join_queries<T, PLANES><<<j.nq, 256, 0, st>>>(dq, p.splits, j.nq, j.dims, (double)j.scale, maxima, l.gsum, l.gsums,
+                                                  w, j.row_stride, j.targets, j.nrows, static_cast<T *>(j.dqueries));
     launches++;
   }
   return op_launched("softmax loss gradient", launches);

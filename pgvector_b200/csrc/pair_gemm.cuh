@@ -158,9 +158,11 @@ struct BoxStore {
   __device__ __forceinline__ uint8_t *at(uint32_t row, uint32_t chunk) const {
     return box + row * 128 + ((chunk ^ (row & 7)) << 4);
   }
-  // Before the box is filled again: what was stored from it has been read.
+  // Before the box is filled again: what was stored from it has been read (all
+  // but the warp's last LATER stores have).
+  template <int LATER = 0>
   __device__ __forceinline__ void reuse() {
-    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LATER) : "memory");
     __syncwarp();
   }
   __device__ __forceinline__ void put(uint32_t chunk, uint4 v) {
