@@ -350,7 +350,17 @@ def search_typed(jobs):
     return out
 
 
-from .ops import matmul_blocks, quantize_blocks, softmax_loss, softmax_loss_grad  # noqa: E402
+_OPS = ('softmax_loss', 'softmax_loss_grad', 'quantize_blocks', 'matmul_blocks')
+
+
+def __getattr__(name):
+    """The operators, on first use: ops.py needs torch, the rest only where it is called."""
+    if name in _OPS:
+        from . import ops
+        globals().update({n: getattr(ops, n) for n in _OPS})
+        return globals()[name]
+    raise AttributeError('module %r has no attribute %r' % (__name__, name))
+
 
 __all__ = ['softmax_loss', 'softmax_loss_grad', 'quantize_blocks', 'matmul_blocks', 'BF16',
            'Shard', 'search_typed', 'merge_topk', 'bitmap_rows', 'bitmap_rows_static', 'backend', 'search_gathered', 'device_count', 'load', 'check',

@@ -26,7 +26,7 @@
 namespace annb200 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033e-8f;   // log2(e), and what FP32 leaves of it
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial maxima and sums, at most about
 constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece, where a piece has 8,192 rows by then
@@ -368,7 +368,10 @@ struct LogitsOp : PairNoHelpers {
       } else {
         // G; columns past the rows go to the buffer's end, which is not read
         const bool kept = valid && has_target(row.target, p.nrows);
-        const float lse2 = row.lse * kLog2e, g = kept ? row.grad / unit * kGradScale : 0.0f;
+        // p = exp2(l2 - lse2) c: c is what rounding lse2 (the lse in base 2) lost
+        const float lse2 = row.lse * kLog2e;
+        const float c = exp2f(-(fmaf(row.lse, kLog2e, -lse2) + row.lse * kLog2eLow));
+        const float g = kept ? row.grad / unit * kGradScale * c : 0.0f, one = 1.0f / c;
         const f32x2 kk = pack2(k, k), zz = pack2(-lse2, -lse2), gg = pack2(g, g);
 #pragma unroll
         for (int j = 0; j < 64; j++) {
@@ -379,7 +382,7 @@ struct LogitsOp : PairNoHelpers {
         if (hit) {
 #pragma unroll
           for (int j = 0; j < 64; j++)
-            v[j] = add2(v[j], pack2(at == 2 * j ? -1.0f : 0.0f, at == 2 * j + 1 ? -1.0f : 0.0f));
+            v[j] = add2(v[j], pack2(at == 2 * j ? -one : 0.0f, at == 2 * j + 1 ? -one : 0.0f));
         }
 #pragma unroll
         for (int j = 0; j < 64; j++) v[j] = mul2(v[j], gg);

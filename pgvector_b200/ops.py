@@ -14,15 +14,14 @@ arguments raise AnnB200Error (ANN_INVALID).
 import contextlib
 import ctypes
 
+import torch
+
 from . import _abi
 from ._lib import AnnB200Error, INVALID, check, load
 
 BLOCK = 128
-
-
-def _types():
-    import torch
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 5}
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 5}
+E4M3 = (torch.float8_e4m3fn, torch.uint8)
 
 
 def _need(ok, message, *args):
@@ -32,66 +31,71 @@ def _need(ok, message, *args):
 
 def _matrix(t, name, dtypes, like=None):
     """A CUDA matrix whose rows are contiguous; its row stride in elements."""
-    import torch
-    _need(isinstance(t, torch.Tensor) and t.dim() == 2, '%s: not a matrix', name)
-    _need(t.dtype in dtypes, '%s: type %s', name, t.dtype)
-    _need(t.is_cuda, '%s: not a CUDA tensor', name)
+    if not (isinstance(t, torch.Tensor) and t.dim() == 2 and t.dtype in dtypes and t.is_cuda):
+        _need(isinstance(t, torch.Tensor) and t.dim() == 2, '%s: not a matrix', name)
+        _need(t.dtype in dtypes, '%s: type %s', name, t.dtype)
+        _need(False, '%s: not a CUDA tensor', name)
     _need(like is None or t.device == like.device, '%s: on another device', name)
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, '%s: its rows are not contiguous', name)
-    if t.shape[0] <= 1:
-        return max(t.stride(0), t.shape[1])
-    _need(t.stride(0) >= t.shape[1], '%s: its rows overlap', name)
-    return t.stride(0)
+    m, n = t.shape
+    stride, inner = t.stride()
+    _need(n <= 1 or inner == 1, '%s: its rows are not contiguous', name)
+    if m <= 1:
+        return max(stride, n)
+    _need(stride >= n, '%s: its rows overlap', name)
+    return stride
 
 
 def _vector(t, name, n, dtype, like):
-    import torch
-    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and tuple(t.shape) == (n,) and t.device == like.device
+    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == (n,) and t.device == like.device
           and t.is_contiguous(), '%s: not a contiguous %s [%d] on the operands\' device', name, dtype, n)
     return t.data_ptr()
 
 
 @contextlib.contextmanager
-def _call(stream, *tensors):
-    """The operands' device made current, and `stream` where one is given: what
-    is allocated inside belongs to it, and operands made on another stream are
-    kept from reuse until its work is done."""
-    import torch
-    device = tensors[0].device
+def _elsewhere(device, stream, tensors):
     with torch.cuda.device(device):
         current = torch.cuda.current_stream(device)
         if stream is None or stream == current:
-            yield ctypes.c_void_p(current.cuda_stream)
+            yield current.cuda_stream
             return
         _need(stream.device == device, 'the stream is of another device')
         with torch.cuda.stream(stream):
-            yield ctypes.c_void_p(stream.cuda_stream)
+            yield stream.cuda_stream
         for t in tensors:
             if t is not None:
                 t.record_stream(stream)
 
 
+def _run(stream, tensors, call):
+    """call(raw stream) with the operands' device current and, where one is given,
+    `stream` as torch's: what call allocates belongs to it, and operands made on
+    another stream are kept from reuse until its work is done."""
+    device = tensors[0].device
+    if stream is None and torch.cuda.current_device() == device.index:
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
+    with _elsewhere(device, stream, tensors) as st:
+        return call(st)
+
+
 def _loss_job(queries, rows, targets, scale):
-    import torch
-    types = _types()
-    job = _abi.AnnB200LossJob()
-    job.row_stride = _matrix(rows, 'rows', types)
-    job.query_stride = _matrix(queries, 'queries', (rows.dtype,), rows)
-    _need(queries.shape[1] == rows.shape[1], 'queries of %d dimensions, rows of %d', queries.shape[1], rows.shape[1])
-    job.dtype, job.dims, job.nq, job.nrows = types[rows.dtype], rows.shape[1], queries.shape[0], rows.shape[0]
-    job.scale = float(scale)
-    job.queries, job.rows = queries.data_ptr(), rows.data_ptr()
-    job.targets = _vector(targets, 'targets', queries.shape[0], torch.int64, rows)
-    return job
+    row_stride = _matrix(rows, 'rows', TYPES)
+    query_stride = _matrix(queries, 'queries', (rows.dtype,), rows)
+    nq, dims = queries.shape
+    _need(dims == rows.shape[1], 'queries of %d dimensions, rows of %d', dims, rows.shape[1])
+    return _abi.AnnB200LossJob(
+        TYPES[rows.dtype], dims, nq, scale, rows.shape[0], queries.data_ptr(), query_stride, rows.data_ptr(),
+        row_stride, _vector(targets, 'targets', nq, torch.int64, rows))
 
 
-def _run_loss(fn, which, job, device, st):
-    import torch
-    need = (ctypes.c_uint64(), ctypes.c_uint64())
-    check(load().AnnB200SoftmaxLossWorkspace(ctypes.byref(job), ctypes.byref(need[0]), ctypes.byref(need[1])))
-    ws = torch.empty((max(need[which].value, 1),), dtype=torch.uint8, device=device)
-    job.workspace, job.workspace_bytes = ws.data_ptr(), ws.numel()
-    check(fn(ctypes.byref(job), st))
+def _workspace(job, which, device):
+    """Room for the call, held by the tensor that is returned."""
+    need = (ctypes.c_uint64 * 2)()
+    at = ctypes.addressof(need)
+    check(load().AnnB200SoftmaxLossWorkspace(ctypes.byref(job), ctypes.cast(at, ctypes.POINTER(ctypes.c_uint64)),
+                                             ctypes.cast(at + 8, ctypes.POINTER(ctypes.c_uint64))))
+    ws = torch.empty((need[which],), dtype=torch.uint8, device=device)
+    job.workspace, job.workspace_bytes = ws.data_ptr(), need[which]
+    return ws
 
 
 def softmax_loss(queries, rows, targets, scale=1.0, status=None, stream=None):
@@ -101,16 +105,20 @@ def softmax_loss(queries, rows, targets, scale=1.0, status=None, stream=None):
     (float32, float16, bfloat16); targets int64 [nq], negative for none (loss
     0). status: optional int32 [nq], ANN_INVALID for a target >= n (loss NaN).
     Returns (loss, lse), float32 [nq]."""
-    import torch
     job = _loss_job(queries, rows, targets, scale)
+    nq, device = queries.shape[0], rows.device
     if status is not None:
-        job.status = _vector(status, 'status', queries.shape[0], torch.int32, rows)
-    with _call(stream, queries, rows, targets, status) as st:
-        loss = torch.empty((queries.shape[0],), dtype=torch.float32, device=rows.device)
-        lse = torch.empty_like(loss)
-        job.loss, job.lse = loss.data_ptr(), lse.data_ptr()
-        _run_loss(load().AnnB200SoftmaxLoss, 0, job, rows.device, st)
-    return loss, lse
+        job.status = _vector(status, 'status', nq, torch.int32, rows)
+
+    def call(st):
+        out = torch.empty((2, nq), dtype=torch.float32, device=device)
+        job.loss = out.data_ptr()
+        job.lse = job.loss + 4 * nq if nq else job.loss
+        ws = _workspace(job, 0, device)  # noqa: F841
+        check(load().AnnB200SoftmaxLoss(ctypes.byref(job), st))
+        return out[0], out[1]
+
+    return _run(stream, (queries, rows, targets, status), call)
 
 
 def softmax_loss_grad(queries, rows, targets, lse, grad=None, scale=1.0, need_queries=True, need_rows=True,
@@ -120,20 +128,26 @@ def softmax_loss_grad(queries, rows, targets, lse, grad=None, scale=1.0, need_qu
     default ones. Returns (dqueries, drows) of the operands' type; None for one
     that is not needed. With torch.autograd in the encoder:
     ``queries.backward(dqueries)``."""
-    import torch
     job = _loss_job(queries, rows, targets, scale)
-    job.lse = _vector(lse, 'lse', queries.shape[0], torch.float32, rows)
+    nq, device = queries.shape[0], rows.device
+    job.lse = _vector(lse, 'lse', nq, torch.float32, rows)
     if grad is not None:
-        job.grad = _vector(grad, 'grad', queries.shape[0], torch.float32, rows)
-    with _call(stream, queries, rows, targets, lse, grad) as st:
-        dq = torch.empty(queries.shape, dtype=rows.dtype, device=rows.device) if need_queries else None
-        dr = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device) if need_rows else None
-        job.dqueries = dq.data_ptr() if need_queries else None
-        job.drows = dr.data_ptr() if need_rows else None
-        if queries.shape[0] == 0 and need_rows:
-            dr.zero_()
-        _run_loss(load().AnnB200SoftmaxLossGrad, 1, job, rows.device, st)
-    return dq, dr
+        job.grad = _vector(grad, 'grad', nq, torch.float32, rows)
+
+    def call(st):
+        dq = torch.empty(queries.shape, dtype=rows.dtype, device=device) if need_queries else None
+        dr = torch.empty(rows.shape, dtype=rows.dtype, device=device) if need_rows else None
+        if need_queries:
+            job.dqueries = dq.data_ptr()
+        if need_rows:
+            job.drows = dr.data_ptr()
+            if nq == 0:
+                dr.zero_()
+        ws = _workspace(job, 1, device)  # noqa: F841
+        check(load().AnnB200SoftmaxLossGrad(ctypes.byref(job), st))
+        return dq, dr
+
+    return _run(stream, (queries, rows, targets, lse, grad), call)
 
 
 def quantize_blocks(x, square=False, stream=None):
@@ -141,28 +155,31 @@ def quantize_blocks(x, square=False, stream=None):
     per 1 x 128 block of a row, or per 128 x 128 block (square). Returns
     (codes float8_e4m3fn [m, k], a view of rows of a multiple of 16 bytes;
     scales float32 [m or ceil(m/128), ceil(k/128)])."""
-    import torch
-    stride = _matrix(x, 'x', _types())
+    stride = _matrix(x, 'x', TYPES)
     m, k = x.shape
-    with _call(stream, x) as st:
-        codes = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=x.device)
+    pad = (k + 15) // 16 * 16
+
+    def call(st):
+        codes = torch.empty((m, pad), dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty(((m + BLOCK - 1) // BLOCK if square else m, (k + BLOCK - 1) // BLOCK),
                              dtype=torch.float32, device=x.device)
-        check(load().AnnB200QuantizeBlocks(_types()[x.dtype], x.data_ptr(), stride, m, k, int(bool(square)),
-                                           codes.data_ptr(), codes.shape[1], scales.data_ptr(), st))
-    return codes[:, :k], scales
+        check(load().AnnB200QuantizeBlocks(TYPES[x.dtype], x.data_ptr(), stride, m, k, int(bool(square)),
+                                           codes.data_ptr(), pad, scales.data_ptr(), st))
+        return codes if pad == k else codes[:, :k], scales
+
+    return _run(stream, (x,), call)
 
 
 def _operand(codes, scales, name, like=None):
     """(row stride in bytes, whether its blocks are square) of an E4M3 operand."""
-    import torch
-    stride = _matrix(codes, name, (torch.float8_e4m3fn, torch.uint8), like)
-    if codes.shape[0] <= 1:
+    stride = _matrix(codes, name, E4M3, like)
+    m, k = codes.shape
+    if m <= 1:
         stride = (stride + 15) // 16 * 16
-    m, kb = codes.shape[0], (codes.shape[1] + BLOCK - 1) // BLOCK
+    kb, tall = (k + BLOCK - 1) // BLOCK, (m + BLOCK - 1) // BLOCK
     _need(isinstance(scales, torch.Tensor) and scales.dtype == torch.float32 and scales.device == codes.device
-          and scales.is_contiguous() and tuple(scales.shape) in ((m, kb), ((m + BLOCK - 1) // BLOCK, kb)),
-          '%s: scales are not a contiguous float32 [%d or %d, %d] on its device', name, m, (m + BLOCK - 1) // BLOCK, kb)
+          and scales.is_contiguous() and scales.shape in ((m, kb), (tall, kb)),
+          '%s: scales are not a contiguous float32 [%d or %d, %d] on its device', name, m, tall, kb)
     return stride, int(scales.shape[0] != m)
 
 
@@ -172,15 +189,18 @@ def matmul_blocks(a, a_scales, b, b_scales, dtype=None, stream=None):
     (rows a multiple of 16 bytes apart, 16-byte aligned). Each side's scales
     have one row per row, or one per 128 rows (square blocks). dtype: float32
     (default), float16 or bfloat16. Returns [m, n]."""
-    import torch
     dtype = dtype or torch.float32
-    _need(dtype in _types(), 'output type %s', dtype)
+    _need(dtype in TYPES, 'output type %s', dtype)
     sa, qa = _operand(a, a_scales, 'a')
     sb, qb = _operand(b, b_scales, 'b', a)
-    _need(a.shape[1] == b.shape[1], 'a has %d columns, b %d', a.shape[1], b.shape[1])
-    m, n, k = a.shape[0], b.shape[0], a.shape[1]
-    with _call(stream, a, a_scales, b, b_scales) as st:
+    m, k = a.shape
+    n = b.shape[0]
+    _need(k == b.shape[1], 'a has %d columns, b %d', k, b.shape[1])
+
+    def call(st):
         out = torch.empty((m, n), dtype=dtype, device=a.device)
         check(load().AnnB200MatmulBlocks(a.data_ptr(), sa, a_scales.data_ptr(), qa, b.data_ptr(), sb,
-                                         b_scales.data_ptr(), qb, m, n, k, _types()[dtype], out.data_ptr(), n, st))
-    return out
+                                         b_scales.data_ptr(), qb, m, n, k, TYPES[dtype], out.data_ptr(), n, st))
+        return out
+
+    return _run(stream, (a, a_scales, b, b_scales), call)
