@@ -511,7 +511,7 @@ struct WideOp {
   static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2, ACCS = 2;
   using Scales = ScaleStage<128, UNIFORM ? 2 : 256, std::conditional_t<UNIFORM, InOrder, PatchOrder>>;
   static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024;
-  static constexpr int SCRATCH = SCALE_BYTES + kPairEpi * kBoxBytes;
+  static constexpr int SCRATCH = SCALE_BYTES + kPairEpi * kBoxBytes;   // (a second box a warp costs a stage: slower)
   using Args = BlocksArgs<T>;
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
   static __device__ __forceinline__ PairItem item(const Args &p, uint32_t i) {
@@ -543,8 +543,8 @@ struct WideOp {
     Scales scales{scratch};
     BoxStore box{scratch + SCALE_BYTES + warp * kBoxBytes};
     for (uint32_t i = cluster; i < items(p); i += clusters) {
-      // UNIFORM: v[c] column c of the lane's row. Else v[32 c + 4 g + u], c = 2 h + l: rows 16 l + lane / 4 (u < 2)
-      // and + 8, columns 64 h + 8 g + 2 (lane % 4) + u % 2
+      // UNIFORM: v[c] column c of the lane's row. Else v[16 c + 4 g + u], c = 2 h + l: rows 16 l + lane / 4 (u < 2)
+      // and + 8, columns 32 h + 8 g + 2 (lane % 4) + u % 2
       float v[128];
 #pragma unroll
       for (int j = 0; j < 128; j++) v[j] = 0.0f;
@@ -553,55 +553,55 @@ struct WideOp {
         const uint32_t scale = scales.take(b, sums);
         const uint32_t addr = sums.acquire() + half * 128;
         if (sums.ok) {
-          constexpr int DEEP = UNIFORM ? 2 : 1;   // reads ahead, where registers allow
-          uint32_t r[DEEP][32];
-          auto read = [&](int c, uint32_t(&to)[32]) {
+          // eight (UNIFORM: four) reads of tensor memory, one ahead of what uses it
+          constexpr int STEP = UNIFORM ? 32 : 16, STEPS = 128 / STEP;
+          uint32_t r[2][STEP];
+          auto read = [&](int c, uint32_t(&to)[STEP]) {
             if constexpr (UNIFORM) TMEM_LD32(addr + c * 32, to);
-            else TMEM_LD_16X64(addr + (c >> 1) * 64 + ((uint32_t)(c & 1) << 20), to);
+            else TMEM_LD_16X32(addr + (c >> 1) * 32 + ((uint32_t)(c & 1) << 20), to);
+          };
+          auto wait = [&](uint32_t(&to)[STEP]) {
+            tmem_ld_wait();
+            if constexpr (UNIFORM) TMEM_KEEP32(to);
+            else TMEM_KEEP16(to);
           };
           read(0, r[0]);
           float rows[4];
-          f32x2 cols[8];
-          if constexpr (UNIFORM)
+          f32x2 cols[16];
+          if constexpr (UNIFORM) {
             rows[0] = shared_float(scale + (quad * 32 + lane) * 4) * shared_float(scale + (128 + half) * 4);
-          else shared_float4(scale + (quad * 32 + (lane >> 2) * 4) * 4, rows);
-          tmem_ld_wait();
-          TMEM_KEEP32(r[0]);
+          } else {
+            shared_float4(scale + (quad * 32 + (lane >> 2) * 4) * 4, rows);
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            if (DEEP == 2 && c < 3) read(c + 1, r[(c + 1) % DEEP]);
-            const uint32_t(&t)[32] = r[c % DEEP];
+            for (int k = 0; k < 8; k++)
+              asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
+                           : "=l"(cols[2 * k]), "=l"(cols[2 * k + 1])
+                           : "r"(scale + (128 + half * 144 + (lane & 3) * 36 + 4 * k) * 4));
+          }
+          wait(r[0]);
+#pragma unroll
+          for (int c = 0; c < STEPS; c++) {
+            if (c + 1 < STEPS) read(c + 1, r[(c + 1) & 1]);
+            const uint32_t(&t)[STEP] = r[c & 1];
             if constexpr (UNIFORM) {
 #pragma unroll
               for (int j = 0; j < 32; j++) v[c * 32 + j] = fmaf(__uint_as_float(t[j]), rows[0], v[c * 32 + j]);
             } else {
-              if ((c & 1) == 0) {   // 64 columns' scales: 16 a thread
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
-                               : "=l"(cols[2 * k]), "=l"(cols[2 * k + 1])
-                               : "r"(scale + (128 + half * 144 + (lane & 3) * 36 + (c >> 1) * 16 + 4 * k) * 4));
-                }
-              }
               const f32x2 ra = pack2(rows[2 * (c & 1)], rows[2 * (c & 1)]);
               const f32x2 rb = pack2(rows[2 * (c & 1) + 1], rows[2 * (c & 1) + 1]);
 #pragma unroll
-              for (int g = 0; g < 8; g++) {
-                float *o4 = v + c * 32 + g * 4;
+              for (int g = 0; g < 4; g++) {
+                float *o4 = v + c * 16 + g * 4;
                 float a0, a1, b0, b1;
-                unpack2(mul2(cols[g], ra), a0, a1);
-                unpack2(mul2(cols[g], rb), b0, b1);
+                unpack2(mul2(cols[(c >> 1) * 4 + g], ra), a0, a1);
+                unpack2(mul2(cols[(c >> 1) * 4 + g], rb), b0, b1);
                 o4[0] = fmaf(__uint_as_float(t[4 * g]), a0, o4[0]);
                 o4[1] = fmaf(__uint_as_float(t[4 * g + 1]), a1, o4[1]);
                 o4[2] = fmaf(__uint_as_float(t[4 * g + 2]), b0, o4[2]);
                 o4[3] = fmaf(__uint_as_float(t[4 * g + 3]), b1, o4[3]);
               }
             }
-            if (c < 3) {
-              if (DEEP == 1) read(c + 1, r[0]);
-              tmem_ld_wait();
-              TMEM_KEEP32(r[(c + 1) % DEEP]);
-            }
+            if (c + 1 < STEPS) wait(r[(c + 1) & 1]);
           }
         }
         sums.release();
@@ -632,7 +632,7 @@ struct WideOp {
               for (int g = 0; g < 4; g++)
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                  const float *q = v + (2 * (x / 2) + u / 2) * 32 + ((x & 1) * 4 + g) * 4 + 2 * (u & 1);
+                  const float *q = v + (2 * x + u / 2) * 16 + g * 4 + 2 * (u & 1);
                   const uint32_t at = (g * 8 + 2 * (lane & 3)) * 4;
                   *reinterpret_cast<float2 *>(box.at(8 * u + lane / 4, at >> 4) + (at & 15)) = make_float2(q[0], q[1]);
                 }
@@ -643,7 +643,7 @@ struct WideOp {
                 uint32_t q[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                  const float *w2 = v + (2 * x + u / 2) * 32 + g * 4 + 2 * (u & 1);
+                  const float *w2 = v + (2 * (2 * x + g / 4) + u / 2) * 16 + (g & 3) * 4 + 2 * (u & 1);
                   q[u] = pack16<T>(w2[0], w2[1]);
                 }
                 asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
@@ -665,15 +665,15 @@ struct WideOp {
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; c++)
+        for (int c = 0; c < 8; c++)
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             const uint32_t m = m0 + 16 * (c & 1) + 8 * (u / 2) + lane / 4;
             if (m >= o.m) continue;
 #pragma unroll
-            for (int g = 0; g < 8; g++) {
-              const uint32_t n = n0 + 64 * (c / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
-              if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[c * 32 + 4 * g + u]);
+            for (int g = 0; g < 4; g++) {
+              const uint32_t n = n0 + 32 * (c / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
+              if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[c * 16 + 4 * g + u]);
             }
           }
       }

@@ -86,17 +86,13 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])    \
       : "r"(taddr))
 
-// 16 lanes x 64 columns: thread t gets, for each 8 columns c (registers 4 (c /
-// 8) ..), lane t / 4 at columns 2 (t % 4) and + 1, then lane t / 4 + 8 at those.
-#define TMEM_LD_16X64(taddr, r)                                                                      \
-  asm volatile(                                                                                      \
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15," \
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                     \
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),        \
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),    \
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), \
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), \
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])                                         \
+// 16 lanes x 32 columns: thread t gets, for each 8 columns c (registers c / 2
+// ..), lane t / 4 at columns 2 (t % 4) and + 1, then lane t / 4 + 8 at those.
+#define TMEM_LD_16X32(taddr, r)                                                                                 \
+  asm volatile(                                                                                                 \
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"   \
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),         \
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])    \
       : "r"(taddr))
 
 // Ties registers that a read of tensor memory fills to the wait before it: what
