@@ -400,7 +400,7 @@ __device__ __forceinline__ bool scales_vec(const Operands &o) {
 template <int COLS, typename T>
 struct NarrowOp {
   static constexpr PairKind KIND = PAIR_E4M3;
-  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr bool A_MN = false, B_MN = false, A_SAME = false;
   static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2;
   // a block's sum passes from role to role in about 1,000 clocks, in which b's next blocks arrive
   static constexpr int ACCS = 2 * COLS >= 128 ? 4 : 8;
@@ -507,7 +507,7 @@ __device__ __forceinline__ void shared_float4(uint32_t addr, float (&v)[4]) {
 template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;
-  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr bool A_MN = false, B_MN = false, A_SAME = false;
   static constexpr int PLANES = 1, MAX_STAGES = 12, CHUNK = 1, HELPERS = 2, ACCS = 2;
   using Scales = ScaleStage<128, UNIFORM ? 2 : 256, std::conditional_t<UNIFORM, InOrder, PatchOrder>>;
   static constexpr int SCALE_BYTES = (Scales::BYTES + 1023) / 1024 * 1024;

@@ -233,11 +233,15 @@ template <> __device__ __forceinline__ uint32_t round2<__half>(f32x2 v, f32x2 &k
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Tiles of 256 queries x 256 rows. GRAD: G of a piece; else the partial sums.
-template <PairKind KIND_, int PLANES_, bool GRAD, typename O>
+// Tiles of 256 queries x 256 rows, 128 columns a thread. GRAD: G of a piece; else
+// the partial sums. FEW: up to 128 queries, which both CTAs multiply with all 256
+// rows; each takes the results of half of them, 64 columns a thread, where one
+// would have had nothing to do.
+template <PairKind KIND_, int PLANES_, bool GRAD, bool FEW, typename O>
 struct LogitsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
-  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr bool A_MN = false, B_MN = false, A_SAME = FEW;
+  static constexpr int COLS = FEW ? 64 : 128, PARTS = 256 / COLS;   // columns a thread; partial sums a tile
   static constexpr int PLANES = PLANES_, SCRATCH = GRAD ? 2 * kPairEpi * kBoxBytes : 0, MAX_STAGES = 8;
   static constexpr int CHUNK = PLANES == 2 ? 2 : 6;   // 24 steps of the tensor cores
   struct Args {
@@ -250,11 +254,11 @@ struct LogitsOp : PairNoHelpers {
     const float *xscale;     // PLANES 2: per query
     const Maxima *maxima;
     const int64_t *targets;
-    float2 *part;            // forward: [query - q0][2 nt]
+    float2 *part;            // forward: [query - q0][PARTS nt]
     float *tlogit;           // [query]
     const float *lse, *grad;
     CUtensorMap g[PLANES];   // gradient: G of the piece
-    float *gsum;             // [query][gsums]: the stored G summed over a half tile, of all pieces
+    float *gsum;             // [query][gsums = PARTS x all row tiles]: the stored G, summed
     uint32_t gsums;
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
@@ -268,7 +272,7 @@ struct LogitsOp : PairNoHelpers {
     float lse, grad, xscale;
   };
   static __device__ __forceinline__ uint32_t query_of(const PairItem &w, uint32_t rank) {
-    return (uint32_t)w.a_row + rank * 128 + ((threadIdx.x >> 5) & 3) * 32 + (threadIdx.x & 31);
+    return (uint32_t)w.a_row + (FEW ? 0 : rank * 128) + ((threadIdx.x >> 5) & 3) * 32 + (threadIdx.x & 31);
   }
   static __device__ __forceinline__ Row row_of(const Args &p, uint32_t i, uint32_t rank) {
     Row r = {-1, 0.0f, 0.0f, 1.0f};
@@ -285,7 +289,8 @@ struct LogitsOp : PairNoHelpers {
   }
   static __device__ __forceinline__ void epilogue(const Args &p, PairSums &sums, uint8_t *scratch, uint32_t rank,
                                                   uint32_t cluster, uint32_t clusters) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t share = (FEW ? 2 * rank : 0) + (warp >> 2);   // which columns of a tile
     const double scale2 = PLANES == 2 ? p.scale2 * (double)undo_scale(p.maxima->all_rows) : p.scale2;
     const float unit = GRAD ? grad_unit(p.maxima) : 1.0f;
     BoxStore box{scratch + 2 * warp * kBoxBytes};
@@ -297,33 +302,33 @@ struct LogitsOp : PairNoHelpers {
       next = row_of(p, i + clusters, rank);
       const uint32_t q = query_of(w, rank);
       const bool valid = q < p.nq;
-      const int64_t col0 = (int64_t)w.b_row + half * 128;   // this thread's first row of W
-      f32x2 v[64];
-      sums.template total<CHUNK, 4>(half * 128, w.kblocks, v);
+      const int64_t col0 = (int64_t)w.b_row + share * COLS;   // this thread's first row of W
+      f32x2 v[COLS / 2];
+      sums.template total<CHUNK, COLS / 32>(share * COLS, w.kblocks, v);
       if (!__any_sync(0xffffffffu, valid)) continue;
       float k = PLANES == 2 ? (float)(scale2 * (double)row.xscale) : (float)scale2;
       if (k == 0.0f) k = FLT_MIN;   // (0 would make NaNs of the infinities that stand for no column)
       const int64_t left = (int64_t)p.nrows - col0;         // columns that are rows of W
-      // the target's column, 128 where it is not here
+      // the target's column, COLS where it is not here
       const int64_t rel = row.target - col0;
-      const int at = valid && rel >= 0 && rel < 128 ? (int)rel : 128;
-      const bool hit = __any_sync(0xffffffffu, at < 128);
-      float s = 0.0f;                                       // of this thread's 128 columns
+      const int at = valid && rel >= 0 && rel < COLS ? (int)rel : COLS;
+      const bool hit = __any_sync(0xffffffffu, at < COLS);
+      float s = 0.0f;                                       // of this thread's columns
       if (!GRAD) {
         if (hit) {
           float t = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 64; j++) {
+          for (int j = 0; j < COLS / 2; j++) {
             float a, b;
             unpack2(v[j], a, b);
             t = at == 2 * j ? a : (at == 2 * j + 1 ? b : t);
           }
-          if (at < 128) p.tlogit[q] = t * k;
+          if (at < COLS) p.tlogit[q] = t * k;
         }
-        if (left < 128) {   // columns past the rows count for nothing
+        if (left < COLS) {   // columns past the rows count for nothing
           const float none = k < 0.0f ? INFINITY : -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 64; j++) {
+          for (int j = 0; j < COLS / 2; j++) {
             float a, b;
             unpack2(v[j], a, b);
             v[j] = pack2(2 * j < (int)left ? a : none, 2 * j + 1 < (int)left ? b : none);
@@ -335,14 +340,14 @@ struct LogitsOp : PairNoHelpers {
         top[0] = top[1] = top[2] = top[3] = start;
         if (k < 0.0f) {
 #pragma unroll
-          for (int j = 0; j < 64; j++) {
+          for (int j = 0; j < COLS / 2; j++) {
             float a, b;
             unpack2(v[j], a, b);
             top[j & 3] = min3(top[j & 3], a, b);
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 64; j++) {
+          for (int j = 0; j < COLS / 2; j++) {
             float a, b;
             unpack2(v[j], a, b);
             top[j & 3] = max3(top[j & 3], a, b);
@@ -355,7 +360,7 @@ struct LogitsOp : PairNoHelpers {
         const f32x2 kk = pack2(k, k), bb = pack2(-base, -base);
         f32x2 e[4] = {};
 #pragma unroll
-        for (int j = 0; j < 64; j++) {
+        for (int j = 0; j < COLS / 2; j++) {
           float a, b;
           unpack2(fma2(v[j], kk, bb), a, b);
           e[j & 3] = add2(e[j & 3], pack2(exp2_approx(a), exp2_approx(b)));
@@ -364,7 +369,7 @@ struct LogitsOp : PairNoHelpers {
         unpack2(add2(add2(e[0], e[1]), add2(e[2], e[3])), a, b);
         s = a + b;
         if (left <= 0) s = 0.0f;
-        if (valid) p.part[(uint64_t)(q - p.q0) * (2 * p.nt) + 2 * w.index + half] = make_float2(m, s);
+        if (valid) p.part[(uint64_t)(q - p.q0) * (PARTS * p.nt) + PARTS * w.index + share] = make_float2(m, s);
       } else {
         // G; columns past the rows go to the buffer's end, which is not read
         const bool kept = valid && has_target(row.target, p.nrows);
@@ -374,25 +379,25 @@ struct LogitsOp : PairNoHelpers {
         const float g = kept ? row.grad / unit * kGradScale * c : 0.0f, one = 1.0f / c;
         const f32x2 kk = pack2(k, k), zz = pack2(-lse2, -lse2), gg = pack2(g, g);
 #pragma unroll
-        for (int j = 0; j < 64; j++) {
+        for (int j = 0; j < COLS / 2; j++) {
           float a, b;
           unpack2(fma2(v[j], kk, zz), a, b);
           v[j] = pack2(exp2_approx(a), exp2_approx(b));
         }
         if (hit) {
 #pragma unroll
-          for (int j = 0; j < 64; j++)
+          for (int j = 0; j < COLS / 2; j++)
             v[j] = add2(v[j], pack2(at == 2 * j ? -one : 0.0f, at == 2 * j + 1 ? -one : 0.0f));
         }
 #pragma unroll
-        for (int j = 0; j < 64; j++) v[j] = mul2(v[j], gg);
+        for (int j = 0; j < COLS / 2; j++) v[j] = mul2(v[j], gg);
         if (!kept) {        // (not 0 times what the query holds)
 #pragma unroll
-          for (int j = 0; j < 64; j++) v[j] = 0;
+          for (int j = 0; j < COLS / 2; j++) v[j] = 0;
         }
-        if (left < 128) {
+        if (left < COLS) {
 #pragma unroll
-          for (int j = 0; j < 64; j++) {
+          for (int j = 0; j < COLS / 2; j++) {
             float a, b;
             unpack2(v[j], a, b);
             v[j] = pack2(2 * j < (int)left ? a : 0.0f, 2 * j + 1 < (int)left ? b : 0.0f);
@@ -404,7 +409,7 @@ struct LogitsOp : PairNoHelpers {
 #pragma unroll
         for (int plane = 0; plane < PLANES; plane++) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
+          for (int h = 0; h < COLS / 64; h++) {
             box.box = scratch + (2 * warp + (turn++ & 1)) * kBoxBytes;   // two boxes in turn
             box.reuse<1>();
 #pragma unroll
@@ -426,7 +431,7 @@ struct LogitsOp : PairNoHelpers {
         float a, b;
         unpack2(add2(sum[0], sum[1]), a, b);
         s = a + b;
-        if (valid) p.gsum[(uint64_t)q * p.gsums + (uint32_t)(p.first / 128) + 2 * w.index + half] = s;
+        if (valid) p.gsum[(uint64_t)q * p.gsums + (uint32_t)(p.first / COLS) + PARTS * w.index + share] = s;
       }
     }
   }
@@ -693,7 +698,9 @@ struct Plan {
   uint32_t ld;             // values a packed row
   bool pack_x, pack_w;
   uint64_t x, w, xscale, maxima, part, tlogit, g, gsum, dq, total;
-  uint32_t nt, chunk;      // forward: row tiles; queries a launch
+  bool few;                // up to 128 queries (LogitsOp)
+  uint32_t parts;          // partial sums a tile
+  uint32_t nt, chunk;      // row tiles; forward: queries a launch
   uint64_t piece;          // gradient: rows a piece
   uint32_t bn, dt, splits; // dimensions a tile, tiles, shares of a piece in dX
 };
@@ -711,9 +718,11 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
   if (p.pack_x) p.x = c.take(nq * p.ld * 2 * p.planes);
   if (p.pack_w) p.w = c.take(j.nrows * p.ld * 2 * p.planes);
   p.nt = (uint32_t)((j.nrows + 255) / 256);
+  p.few = nq <= 128;
+  p.parts = p.few ? 4 : 2;
   if (!grad) {
-    p.chunk = (uint32_t)std::min<uint64_t>(up(nq, 256), std::max<uint64_t>(256, kPartBytes / (16ull * p.nt) / 256 * 256));
-    p.part = c.take(std::min<uint64_t>(nq, p.chunk) * p.nt * 16);
+    p.chunk = (uint32_t)std::min<uint64_t>(up(nq, 256), std::max<uint64_t>(256, kPartBytes / (8ull * p.parts * p.nt) / 256 * 256));
+    p.part = c.take(std::min<uint64_t>(nq, p.chunk) * p.nt * p.parts * 8);
     p.tlogit = c.take(nq * 4);
   } else {
     // a piece: G of kPieceBytes (it stays in L2 for the products that read
@@ -721,7 +730,7 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
     p.piece = std::max<uint64_t>(8192, kPieceBytes / (2 * p.planes * nq) / 256 * 256);
     p.piece = std::min<uint64_t>({p.piece, up(j.nrows, 256), 1u << 20});
     p.g = c.take(nq * p.piece * 2 * p.planes);
-    p.gsum = c.take(nq * 2 * p.nt * 4);
+    p.gsum = c.take(nq * p.parts * p.nt * 4);
     // 128 dimensions a tile where 256 would leave over an eighth of them empty
     const uint64_t full = up(j.dims, 256), fine = up(j.dims, 128);
     p.bn = fine * 8 < full * 7 ? 128 : 256;
@@ -745,7 +754,7 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
 }
 
 // T: the operands' type; O: the products'.
-template <typename T, typename O, PairKind KIND, int PLANES>
+template <typename T, typename O, PairKind KIND, int PLANES, bool FEW>
 int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   const Plan p = plan_of(j, grad);
   const int sms = op_sms();
@@ -821,7 +830,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     l.targets = j.targets;
   };
   if (!grad) {
-    using Op = LogitsOp<KIND, PLANES, false, O>;
+    using Op = LogitsOp<KIND, PLANES, false, FEW, O>;
     typename Op::Args l = {};
     logits(l);
     l.nt = p.nt;
@@ -835,7 +844,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       // (a launch covers whole tiles of queries, except at their end)
       e = launch_pair<Op>(l, l.mt * l.nt, sms, st);
       if (e != cudaSuccess) break;
-      join_sums<<<n, 128, 0, st>>>(l.part, 2 * p.nt, q0, j.nrows, j.targets, l.tlogit, j.loss, j.lse, j.status);
+      join_sums<<<n, 128, 0, st>>>(l.part, p.parts * p.nt, q0, j.nrows, j.targets, l.tlogit, j.loss, j.lse, j.status);
       launches += 2;
     }
     if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss: %s", cudaGetErrorString(e));
@@ -845,7 +854,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   O *g = reinterpret_cast<O *>(ws + p.g);
   float *dq = reinterpret_cast<float *>(ws + p.dq);
   const uint64_t gplane = (uint64_t)j.nq * p.piece;
-  using LOp = LogitsOp<KIND, PLANES, true, O>;
+  using LOp = LogitsOp<KIND, PLANES, true, FEW, O>;
   using QOp = QueriesOp<KIND, PLANES>;
   using ROp = RowsOp<KIND, PLANES, T>;
   typename LOp::Args l = {};
@@ -855,7 +864,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   l.grad = j.grad;
   map(l.g, g, p.piece, j.nq, p.piece, gplane, 32);
   l.gsum = reinterpret_cast<float *>(ws + p.gsum);
-  l.gsums = 2 * p.nt;
+  l.gsums = p.parts * p.nt;
   for (uint64_t first = 0; first < j.nrows && e == cudaSuccess; first += p.piece) {
     const uint64_t n = std::min(p.piece, j.nrows - first);
     l.first = first;
@@ -929,10 +938,11 @@ int run_job(const AnnB200LossJob *j, bool grad, void *stream) {
       j->workspace_bytes < plan_of(*j, grad).total)
     return report_error(OP_INVALID, "workspace too small or not 256-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool few = j->nq <= 128;
   switch (j->dtype) {
-    case ANNB200_F32: return run_loss<float, __half, PAIR_F16, 2>(*j, grad, st);
-    case ANNB200_F16: return run_loss<__half, __half, PAIR_F16, 1>(*j, grad, st);
-    default: return run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1>(*j, grad, st);
+    case ANNB200_F32: return few ? run_loss<float, __half, PAIR_F16, 2, true>(*j, grad, st) : run_loss<float, __half, PAIR_F16, 2, false>(*j, grad, st);
+    case ANNB200_F16: return few ? run_loss<__half, __half, PAIR_F16, 1, true>(*j, grad, st) : run_loss<__half, __half, PAIR_F16, 1, false>(*j, grad, st);
+    default: return few ? run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1, true>(*j, grad, st) : run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1, false>(*j, grad, st);
   }
 }
 

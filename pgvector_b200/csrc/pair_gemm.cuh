@@ -293,12 +293,13 @@ struct PairShape {
 
 // Op: KIND, A_MN, B_MN, PLANES, SCRATCH (bytes), MAX_STAGES (<= 12), CHUNK (K blocks a
 // sum; 0: the item's), ACCS (sums in tensor memory at a time: 512 / ACCS >= bn),
-// HELPERS (0 or 2 warps), Args with maps a[PLANES],
+// A_SAME (both CTAs take the same 128 rows of A), HELPERS (0 or 2 warps), Args with maps a[PLANES],
 // b[PLANES] and bn (columns of a tile), items(args), item(args, i),
 // epilogue(args, sums, scratch, rank, cluster, clusters): all of the cluster's
 // items; init and help where there are helpers.
 struct PairNoHelpers {
   static constexpr int HELPERS = 0, ACCS = 2;
+  static constexpr bool A_SAME = false;
   static __device__ __forceinline__ void init(uint8_t *) {}
   template <class Args>
   static __device__ __forceinline__ void help(const Args &, uint8_t *, uint32_t, uint32_t, uint32_t,
@@ -370,7 +371,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         bool ok = true;
         for (uint32_t i = cluster; i < items && ok; i += clusters) {
           const PairItem w = Op::item(args, i);
-          const int32_t ar = w.a_row + (int32_t)rank * 128, br = w.b_row + (int32_t)(rank * (args.bn / 2));
+          const int32_t ar = w.a_row + (Op::A_SAME ? 0 : (int32_t)rank * 128), br = w.b_row + (int32_t)(rank * (args.bn / 2));
           for (uint32_t kb = 0; kb < w.kblocks; kb++) {
             if (!pair_wait(empty + s, (round & 1) ^ 1, abort)) {
               ok = false;
