@@ -601,7 +601,8 @@ int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
  *   dqueries_i = scale * sum_j G_ij row_j      [nq][dims]
  *   drows_j    = scale * sum_i G_ij query_i    [nrows][dims]
  *
- * dense in dtype, overwritten; either may be NULL. The logits are computed
+ * dense in dtype, overwritten, apart from every input; either may be NULL.
+ * The logits are computed
  * again, piece by piece. Each piece of G is held in 16 bits for FP16 and BF16
  * operands, two FP16 terms for FP32 operands. Results do not depend on timing: no
  * atomics. A non-finite value makes non-finite what the formulas make so.

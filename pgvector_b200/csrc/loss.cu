@@ -29,7 +29,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033e-8f;   // log2(e), and what FP32 leaves of it
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial maxima and sums, at most about
-constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece, where a piece has 8,192 rows by then
+constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece (at 128 MB launches and dX's sums showed: 5 % more)
+constexpr uint64_t kMostPieceBytes = 4ull << 30;
 constexpr uint32_t kPlanClusters = 74;          // clusters the plan splits for (148 SMs)
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -258,7 +259,7 @@ struct LogitsOp : PairNoHelpers {
     float *tlogit;           // [query]
     const float *lse, *grad;
     CUtensorMap g[PLANES];   // gradient: G of the piece
-    float *gsum;             // [query][gsums = PARTS x all row tiles]: the stored G, summed
+    float *gsum;             // [query][gsums = PARTS x a piece's row tiles]: the stored G, summed over pieces
     uint32_t gsums;
   };
   static __device__ __forceinline__ uint32_t items(const Args &p) { return p.mt * p.nt; }
@@ -431,7 +432,10 @@ struct LogitsOp : PairNoHelpers {
         float a, b;
         unpack2(add2(sum[0], sum[1]), a, b);
         s = a + b;
-        if (valid) p.gsum[(uint64_t)q * p.gsums + (uint32_t)(p.first / COLS) + PARTS * w.index + share] = s;
+        if (valid) {   // (the same thread of every piece's tile: added in order)
+          float *sum_at = p.gsum + (uint64_t)q * p.gsums + PARTS * w.index + share;
+          *sum_at = p.first ? *sum_at + s : s;
+        }
       }
     }
   }
@@ -725,12 +729,14 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
     p.part = c.take(std::min<uint64_t>(nq, p.chunk) * p.nt * p.parts * 8);
     p.tlogit = c.take(nq * 4);
   } else {
-    // a piece: G of kPieceBytes (it stays in L2 for the products that read
-    // it), but 8,192 rows at least, since each piece reads and writes dX's sums
-    p.piece = std::max<uint64_t>(8192, kPieceBytes / (2 * p.planes * nq) / 256 * 256);
+    // a piece: G of kPieceBytes, but 8,192 rows at least, since each piece adds
+    // to dX's sums, as long as G stays within kMostPieceBytes
+    const uint64_t row_bytes = 2ull * p.planes * nq;
+    p.piece = std::max<uint64_t>({256, std::min<uint64_t>(8192, kMostPieceBytes / row_bytes / 256 * 256),
+                                  kPieceBytes / row_bytes / 256 * 256});
     p.piece = std::min<uint64_t>({p.piece, up(j.nrows, 256), 1u << 20});
     p.g = c.take(nq * p.piece * 2 * p.planes);
-    p.gsum = c.take(nq * p.parts * p.nt * 4);
+    p.gsum = c.take(nq * p.parts * (p.piece / 256) * 4);
     // 128 dimensions a tile where 256 would leave over an eighth of them empty
     const uint64_t full = up(j.dims, 256), fine = up(j.dims, 128);
     p.bn = fine * 8 < full * 7 ? 128 : 256;
@@ -864,7 +870,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   l.grad = j.grad;
   map(l.g, g, p.piece, j.nq, p.piece, gplane, 32);
   l.gsum = reinterpret_cast<float *>(ws + p.gsum);
-  l.gsums = p.parts * p.nt;
+  l.gsums = (uint32_t)(p.parts * (p.piece / 256));
   for (uint64_t first = 0; first < j.nrows && e == cudaSuccess; first += p.piece) {
     const uint64_t n = std::min(p.piece, j.nrows - first);
     l.first = first;
@@ -940,9 +946,15 @@ int run_job(const AnnB200LossJob *j, bool grad, void *stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool few = j->nq <= 128;
   switch (j->dtype) {
-    case ANNB200_F32: return few ? run_loss<float, __half, PAIR_F16, 2, true>(*j, grad, st) : run_loss<float, __half, PAIR_F16, 2, false>(*j, grad, st);
-    case ANNB200_F16: return few ? run_loss<__half, __half, PAIR_F16, 1, true>(*j, grad, st) : run_loss<__half, __half, PAIR_F16, 1, false>(*j, grad, st);
-    default: return few ? run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1, true>(*j, grad, st) : run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1, false>(*j, grad, st);
+    case ANNB200_F32:
+      return few ? run_loss<float, __half, PAIR_F16, 2, true>(*j, grad, st)
+                 : run_loss<float, __half, PAIR_F16, 2, false>(*j, grad, st);
+    case ANNB200_F16:
+      return few ? run_loss<__half, __half, PAIR_F16, 1, true>(*j, grad, st)
+                 : run_loss<__half, __half, PAIR_F16, 1, false>(*j, grad, st);
+    default:
+      return few ? run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1, true>(*j, grad, st)
+                 : run_loss<__nv_bfloat16, __nv_bfloat16, PAIR_BF16, 1, false>(*j, grad, st);
   }
 }
 

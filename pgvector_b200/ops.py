@@ -83,7 +83,7 @@ def _loss_job(queries, rows, targets, scale):
     nq, dims = queries.shape
     _need(dims == rows.shape[1], 'queries of %d dimensions, rows of %d', dims, rows.shape[1])
     return _abi.AnnB200LossJob(
-        TYPES[rows.dtype], dims, nq, scale, rows.shape[0], queries.data_ptr(), query_stride, rows.data_ptr(),
+        TYPES[rows.dtype], dims, nq, float(scale), rows.shape[0], queries.data_ptr(), query_stride, rows.data_ptr(),
         row_stride, _vector(targets, 'targets', nq, torch.int64, rows))
 
 

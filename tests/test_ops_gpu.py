@@ -114,6 +114,24 @@ def test_loss_and_gradients(cuda, dtype, nq, rows, dims):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+def test_gradients_over_several_pieces_of_the_rows(cuda, dtype):
+    # more than the 512 MB that a piece's part of the logits' gradient takes
+    x, w, t, g = loss_inputs(2100, 140001, 16, dtype, seed=18)
+    check_loss(x, w, t, g, scale=12.5)
+
+
+def test_the_loss_of_a_batch_in_several_launches(cuda):
+    # 1,300 queries against 3,000,001 rows: partial sums for 1,280 queries at a time
+    import torch
+    import pgvector_b200 as pb
+    x, w, t, _ = loss_inputs(1300, 3000001, 16, 'bf16', seed=19)
+    loss, lse = pb.softmax_loss(x, w, t, scale=9.0)
+    for part in (slice(0, 700), slice(700, 1300)):
+        a, b = pb.softmax_loss(x[part], w, t[part].contiguous(), scale=9.0)
+        assert torch.equal(a, loss[part]) and torch.equal(b, lse[part])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 def test_loss_large_and_odd_scales(cuda, dtype):
     x, w, t, g = loss_inputs(40, 900, 72, dtype, seed=3)
     for scale in (0.0, -3.0, 100.0):
@@ -356,6 +374,43 @@ def test_loss_in_captured_graphs(cuda, dtype):
         for _, out in graphs:
             for u, v in zip(out, want):
                 assert torch.equal(u, v)
+
+
+CAPTURE_FIRST = r"""
+import sys
+sys.path.insert(0, %r)
+import torch
+import pgvector_b200 as pb
+x = torch.randn((100, 64), device='cuda')
+w = torch.randn((900, 64), device='cuda')
+t = torch.arange(100, device='cuda')
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    loss, lse = pb.softmax_loss(x, w, t)
+    dx, dw = pb.softmax_loss_grad(x, w, t, lse)
+    a, sa = pb.quantize_blocks(x)
+    b, sb = pb.quantize_blocks(w, square=True)
+    out = [pb.matmul_blocks(a[:m], sa[:m], b, sb) for m in (1, 20, 100)]
+graph.replay()
+torch.cuda.synchronize()
+want = pb.softmax_loss(x, w, t)
+assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+for u, v in zip((dx, dw), pb.softmax_loss_grad(x, w, t, lse)):
+    assert torch.equal(u, v)
+for m, o in zip((1, 20, 100), out):
+    assert torch.equal(o, pb.matmul_blocks(a[:m], sa[:m], b, sb))
+print('captured')
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured(cuda):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, '-c', CAPTURE_FIRST % root], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and 'captured' in out.stdout, out.stderr
 
 
 # ---------------------------------------------------------------- blocks of E4M3
