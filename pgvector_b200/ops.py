@@ -89,12 +89,11 @@ def _loss_job(queries, rows, targets, scale):
 
 def _workspace(job, which, device):
     """Room for the call, held by the tensor that is returned."""
-    need = (ctypes.c_uint64 * 2)()
-    at = ctypes.addressof(need)
-    check(load().AnnB200SoftmaxLossWorkspace(ctypes.byref(job), ctypes.cast(at, ctypes.POINTER(ctypes.c_uint64)),
-                                             ctypes.cast(at + 8, ctypes.POINTER(ctypes.c_uint64))))
-    ws = torch.empty((need[which],), dtype=torch.uint8, device=device)
-    job.workspace, job.workspace_bytes = ws.data_ptr(), need[which]
+    need = (ctypes.c_uint64(), ctypes.c_uint64())
+    check(load().AnnB200SoftmaxLossWorkspace(ctypes.byref(job), ctypes.byref(need[0]), ctypes.byref(need[1])))
+    size = need[which].value
+    ws = torch.empty((size,), dtype=torch.uint8, device=device)
+    job.workspace, job.workspace_bytes = ws.data_ptr(), size
     return ws
 
 
@@ -116,7 +115,7 @@ def softmax_loss(queries, rows, targets, scale=1.0, status=None, stream=None):
         job.lse = job.loss + 4 * nq if nq else job.loss
         ws = _workspace(job, 0, device)  # noqa: F841
         check(load().AnnB200SoftmaxLoss(ctypes.byref(job), st))
-        return out[0], out[1]
+        return out.unbind()
 
     return _run(stream, (queries, rows, targets, status), call)
 
