@@ -698,7 +698,7 @@ cudaError_t launch_tiles(const Operands &o, T *out, bool wide, uint32_t bn, int 
       (!args.boxes ||
        encode_operand_map(&args.map, 2, out, o.n * sizeof(T) / 2, o.m, o.out_stride * sizeof(T), 32));
   if (!maps) return cudaErrorInvalidValue;
-  return launch_pair<Op>(args, args.mt * args.nt, sms, st);
+  return launch_pair<Op>(args, args.mt * args.nt, sms, st, false);
 }
 
 template <typename T>

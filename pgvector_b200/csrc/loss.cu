@@ -93,6 +93,7 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
 __global__ void __launch_bounds__(256) find_maxima(const float *w, uint64_t w_stride, uint64_t nrows, const float *x,
                                                    uint64_t x_stride, uint32_t nq, uint32_t dims, uint32_t tx,
                                                    const int64_t *targets, Maxima *out) {
+  chain_next();
   const bool queries = blockIdx.x >= kRowParts;
   const uint32_t block = queries ? blockIdx.x - kRowParts : blockIdx.x, grid = queries ? kQueryParts : kRowParts;
   const float *from = queries ? x : w;
@@ -168,6 +169,8 @@ __device__ __forceinline__ void pack8(const T *row, uint32_t c, uint32_t dims, b
 }
 template <typename T, typename O, int PLANES>
 __global__ void __launch_bounds__(256) lay_out(const Layout<T, O, PLANES> p) {
+  chain_wait();
+  chain_next();
   uint32_t block = blockIdx.x;
   if (block < p.query_blocks) {   // a warp a query
     const uint32_t lane = threadIdx.x % 32;
@@ -445,6 +448,8 @@ struct LogitsOp : PairNoHelpers {
 __global__ void __launch_bounds__(128) join_sums(const float2 *part, uint32_t n, uint32_t q0, uint64_t nrows,
                                                   const int64_t *targets, const float *tlogit, float *loss, float *lse,
                                                   int32_t *status) {
+  chain_wait();
+  chain_next();
   const uint32_t q = q0 + blockIdx.x;
   part += (uint64_t)blockIdx.x * n;
   __shared__ float top[4];
@@ -632,6 +637,7 @@ __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t 
                                                     double scale, const Maxima *maxima, const float *gsum,
                                                     uint32_t gsums, const T *rows, uint64_t stride,
                                                     const int64_t *targets, uint64_t nrows, T *out) {
+  chain_wait();
   const uint32_t q = blockIdx.x, ld = (dims + 3) / 4 * 4;
   const uint64_t plane = (uint64_t)nq * ld;
   const int64_t t = targets[q];
@@ -812,8 +818,9 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     launches++;
   }
   if (const uint32_t blocks = lay.query_blocks + lay.row_blocks + lay.grad_blocks) {
-    lay_out<T, O, PLANES><<<blocks, 256, 0, st>>>(lay);
+    e = launch_chained(launches > 0, lay_out<T, O, PLANES>, blocks, 256, 0, st, lay);
     launches++;
+    if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss: %s", cudaGetErrorString(e));
   }
   bool maps = true;
   auto map = [&](CUtensorMap *m, const O *base, uint64_t inner, uint64_t outer, uint64_t ld, uint64_t plane,
@@ -843,14 +850,15 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     l.part = reinterpret_cast<float2 *>(ws + p.part);
     l.tlogit = reinterpret_cast<float *>(ws + p.tlogit);
     if (!maps) return report_error(OP_BACKEND_ERROR, "softmax loss: tensor map");
-    for (uint32_t q0 = 0; q0 < j.nq; q0 += p.chunk) {
+    for (uint32_t q0 = 0; q0 < j.nq && e == cudaSuccess; q0 += p.chunk) {
       const uint32_t n = std::min(p.chunk, j.nq - q0);
       l.q0 = q0;
       l.mt = (n + 255) / 256;
       // (a launch covers whole tiles of queries, except at their end)
-      e = launch_pair<Op>(l, l.mt * l.nt, sms, st);
+      e = launch_pair<Op>(l, l.mt * l.nt, sms, st, launches > 0);
       if (e != cudaSuccess) break;
-      join_sums<<<n, 128, 0, st>>>(l.part, p.parts * p.nt, q0, j.nrows, j.targets, l.tlogit, j.loss, j.lse, j.status);
+      e = launch_chained(true, join_sums, n, 128, 0, st, l.part, p.parts * p.nt, q0, j.nrows, j.targets, l.tlogit,
+                         j.loss, j.lse, j.status);
       launches += 2;
     }
     if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss: %s", cudaGetErrorString(e));
@@ -875,7 +883,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     const uint64_t n = std::min(p.piece, j.nrows - first);
     l.first = first;
     l.nt = (uint32_t)((n + 255) / 256);
-    e = maps ? launch_pair<LOp>(l, l.mt * l.nt, sms, st) : cudaErrorInvalidValue;
+    e = maps ? launch_pair<LOp>(l, l.mt * l.nt, sms, st, true) : cudaErrorInvalidValue;
     launches++;
     if (j.dqueries && e == cudaSuccess) {
       typename QOp::Args a = {};
@@ -890,7 +898,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       a.dims = j.dims;
       a.add = first != 0;
       maps = maps && encode_sums_map(&a.part, dq, j.dims, j.nq, p.splits, up(j.dims, 4) * 4);
-      e = maps ? launch_pair<QOp>(a, a.mt * a.nt * a.splits, sms, st) : cudaErrorInvalidValue;
+      e = maps ? launch_pair<QOp>(a, a.mt * a.nt * a.splits, sms, st, true) : cudaErrorInvalidValue;
       launches++;
     }
     if (j.drows && e == cudaSuccess) {
@@ -910,16 +918,16 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
       // (as 16-bit values, whatever T: a box is 128 bytes wide)
       if (a.boxes)
         maps = maps && encode_operand_map(&a.map, 2, a.out, j.dims * sizeof(T) / 2, n, j.dims * sizeof(T), 32);
-      e = maps ? launch_pair<ROp>(a, a.mt * a.nt, sms, st) : cudaErrorInvalidValue;
+      e = maps ? launch_pair<ROp>(a, a.mt * a.nt, sms, st, true) : cudaErrorInvalidValue;
       launches++;
     }
   }
-  if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss gradient: %s", cudaGetErrorString(e));
-  if (j.dqueries) {
-    join_queries<T, PLANES><<<j.nq, 256, 0, st>>>(dq, p.splits, j.nq, j.dims, (double)j.scale, maxima, l.gsum, l.gsums,
-                                                  w, j.row_stride, j.targets, j.nrows, static_cast<T *>(j.dqueries));
+  if (j.dqueries && e == cudaSuccess) {
+    e = launch_chained(true, join_queries<T, PLANES>, j.nq, 256, 0, st, dq, p.splits, j.nq, j.dims, (double)j.scale,
+                       maxima, l.gsum, l.gsums, w, j.row_stride, j.targets, j.nrows, static_cast<T *>(j.dqueries));
     launches++;
   }
+  if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss gradient: %s", cudaGetErrorString(e));
   return op_launched("softmax loss gradient", launches);
 }
 

@@ -53,6 +53,28 @@ inline int op_launched(const char *what, unsigned long long kernels) {
   return OP_OK;
 }
 
+// A call's kernels after its first start while the one before still runs, get
+// their setup done, and wait for its end before they touch memory: short kernels
+// are mostly setup (5 of 8 us of a product of a few tiles). Every kernel of a
+// chain waits, so each starts its work after all before it.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... Params, typename... Args>
+cudaError_t launch_chained(bool after, void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
+                           cudaStream_t st, Args... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // A tensor map of an operand (shard.cu): boxes of 128 bytes x box_rows rows, 128-byte swizzle.
 bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
                         uint64_t pitch, uint32_t box_rows);

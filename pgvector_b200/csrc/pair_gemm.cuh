@@ -357,6 +357,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  chain_wait();
+  chain_next();
 
   if (warp < kPairEpi) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpiRegs));
@@ -481,9 +483,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   }
 }
 
-// One cluster per pair of SMs, or per item where there are fewer.
+// One cluster per pair of SMs, or per item where there are fewer. after: not its call's first kernel.
 template <class Op>
-cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, cudaStream_t st) {
+cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, cudaStream_t st, bool after) {
   const int b_bytes = (int)args.bn * 64;
   const int smem = PairShape<Op>::smem(b_bytes);
   // the attribute is a device's: set once on each
@@ -498,8 +500,7 @@ cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, 
     set.fetch_or(bit, std::memory_order_relaxed);
   }
   const uint32_t clusters = items < (uint32_t)(sms / 2) ? items : (uint32_t)(sms / 2);
-  pair_gemm<Op><<<2 * clusters, kPairThreads, smem, st>>>(args);
-  return cudaGetLastError();
+  return launch_chained(after, pair_gemm<Op>, 2 * clusters, kPairThreads, smem, st, args);
 }
 
 }  // namespace annb200
