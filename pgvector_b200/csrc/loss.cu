@@ -152,27 +152,27 @@ __device__ __forceinline__ void pack8(const T *row, uint32_t c, uint32_t dims, b
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = !zero && c + j < dims ? row[c + j] : from_float<T>(0.0f);
   }
-  if (PLANES == 1) {
+  if constexpr (PLANES == 1) {
     *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<uint4 *>(v);
-    return;
-  }
-  uint32_t hi[4], lo[4];
+  } else {
+    uint32_t hi[4], lo[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    float f[2], l[2];
-    __half h[2];
+    for (int j = 0; j < 4; j++) {
+      float f[2], l[2];
+      __half h[2];
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      f[u] = to_float(v[2 * j + u]) * mul;
-      if (isinf(f[u])) f[u] = NAN;
-      h[u] = __float2half_rn(f[u]);
-      l[u] = isnan(f[u]) ? 0.0f : f[u] - __half2float(h[u]);
+      for (int u = 0; u < 2; u++) {
+        f[u] = to_float(v[2 * j + u]) * mul;
+        if (isinf(f[u])) f[u] = NAN;
+        h[u] = __float2half_rn(f[u]);
+        l[u] = isnan(f[u]) ? 0.0f : f[u] - __half2float(h[u]);
+      }
+      hi[j] = pack16<__half>(f[0], f[1]);
+      lo[j] = pack16<__half>(l[0], l[1]);
     }
-    hi[j] = pack16<__half>(f[0], f[1]);
-    lo[j] = pack16<__half>(l[0], l[1]);
+    *reinterpret_cast<uint4 *>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(out + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  *reinterpret_cast<uint4 *>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-  *reinterpret_cast<uint4 *>(out + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 template <typename T, typename O, int PLANES>
 __global__ void __launch_bounds__(256) lay_out(const Layout<T, O, PLANES> p) {
