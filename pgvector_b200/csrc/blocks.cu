@@ -322,7 +322,7 @@ struct ScaleStage {
   }
   // The helpers' part for one item: t = 0 .. 63; row(c): scale c's row of kb blocks.
   template <typename Rows>
-  __device__ __forceinline__ bool fill(uint32_t t, const Rows &row_of, uint32_t kb, bool vec, volatile uint32_t *abort) {
+  __device__ __forceinline__ bool fill(uint32_t t, const Rows &row_of, uint32_t kb, bool vec, volatile PairBounds *bounds) {
     constexpr int EACH = (LANES + COLS + 63) / 64;
     const float *row[EACH];
 #pragma unroll
@@ -344,7 +344,8 @@ struct ScaleStage {
     load(0);
     for (uint32_t b0 = 0; b0 < kb; b0 += AHEAD, group++) {
       uint64_t *bar = bars() + (group & 1);
-      if (!pair_wait(bar + 2, ((group >> 1) & 1) ^ 1, abort)) return false;
+      // (the warp leaves together: a lane that goes on alone would wait for the others below)
+      if (!__all_sync(0xffffffffu, pair_wait(bar + 2, ((group >> 1) & 1) ^ 1, bounds))) return false;
       float *at = reinterpret_cast<float *>(scratch + (group & 1) * BUFFER);
 #pragma unroll
       for (int e = 0; e < EACH; e++) {
@@ -366,13 +367,14 @@ struct ScaleStage {
   template <typename Sums>
   __device__ __forceinline__ uint32_t take(uint32_t b, Sums &sums) const {
     if (b % AHEAD == 0 && sums.ok)
-      sums.ok = __all_sync(0xffffffffu, pair_wait(bars() + (group & 1), (group >> 1) & 1, sums.abort));
+      sums.ok = __all_sync(0xffffffffu, pair_wait(bars() + (group & 1), (group >> 1) & 1, sums.bounds));
     return smem_u32(scratch) + (group & 1) * BUFFER + (b % AHEAD) * (ROW * 4);
   }
-  __device__ __forceinline__ void done(uint32_t b, uint32_t kb) {
+  // (A warp whose waits have run out no longer keeps step with the others: it does not arrive for them.)
+  __device__ __forceinline__ void done(uint32_t b, uint32_t kb, bool ok) {
     if (b % AHEAD == AHEAD - 1 || b + 1 == kb) {
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(bars() + 2 + (group & 1));
+      if ((threadIdx.x & 31) == 0 && ok) mbar_arrive(bars() + 2 + (group & 1));
       group++;
     }
   }
@@ -419,7 +421,7 @@ struct NarrowOp {
   }
   static __device__ __forceinline__ void init(uint8_t *scratch) { Scales{scratch}.init(); }
   static __device__ __forceinline__ void help(const Args &p, uint8_t *scratch, uint32_t rank, uint32_t cluster,
-                                              uint32_t clusters, volatile uint32_t *abort) {
+                                              uint32_t clusters, volatile PairBounds *bounds) {
     const Operands &o = p.o;
     Scales scales{scratch};
     const bool vec = scales_vec(o);
@@ -431,7 +433,7 @@ struct NarrowOp {
                          return c < 128 ? o.b_scales + (min(n0 + c, o.n - 1) >> o.b_shift) * o.kb
                                         : o.a_scales + (min(m0 + c - 128, o.m - 1) >> o.a_shift) * o.kb;
                        },
-                       o.kb, vec, abort))
+                       o.kb, vec, bounds))
         return;
     }
   }
@@ -471,7 +473,7 @@ struct NarrowOp {
           }
         }
         sums.release();
-        scales.done(b, o.kb);
+        scales.done(b, o.kb, sums.ok);
       }
       const PairItem w = item(p, i);
       const uint64_t n = (uint64_t)w.a_row + rank * 128 + quad * 32 + lane;   // b's row
@@ -528,7 +530,7 @@ struct WideOp {
   }
   static __device__ __forceinline__ void init(uint8_t *scratch) { Scales{scratch}.init(); }
   static __device__ __forceinline__ void help(const Args &p, uint8_t *scratch, uint32_t rank, uint32_t cluster,
-                                              uint32_t clusters, volatile uint32_t *abort) {
+                                              uint32_t clusters, volatile PairBounds *bounds) {
     const Operands &o = p.o;
     Scales scales{scratch};
     const bool vec = scales_vec(o);
@@ -541,7 +543,7 @@ struct WideOp {
                          const uint64_t n = n0 + (UNIFORM ? (c - 128) * 128 : c - 128);
                          return o.b_scales + (min(n, o.n - 1) >> o.b_shift) * o.kb;
                        },
-                       o.kb, vec, abort))
+                       o.kb, vec, bounds))
         return;
     }
   }
@@ -614,7 +616,7 @@ struct WideOp {
           }
         }
         sums.release();
-        scales.done(b, o.kb);
+        scales.done(b, o.kb, sums.ok);
       }
       const PairItem w = item(p, i);
       const uint32_t m0 = (uint32_t)w.a_row + rank * 128 + quad * 32, n0 = (uint32_t)w.b_row + half * 128;

@@ -76,6 +76,9 @@ cudaError_t launch_chained(bool after, void (*kernel)(Params...), unsigned grid,
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// The limit of a pipeline wait (scan_tc.cu).
+uint64_t pipeline_wait_ns();
+
 // A tensor map of an operand (shard.cu): boxes of 128 bytes x box_rows rows, 128-byte swizzle.
 bool encode_operand_map(CUtensorMap *map, uint32_t bytes, const void *base, uint64_t inner, uint64_t outer,
                         uint64_t pitch, uint32_t box_rows);

@@ -129,27 +129,37 @@ __device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap *map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// Wait for a phase, at most kWaitNs and until another role of the CTA has given
+// What bounds a CTA's waits: the flag that a role has given up, and the launch's
+// limit (pipeline_wait_ns), read only after some tries.
+constexpr uint32_t kTryNs = 100000;
+struct PairBounds {
+  uint32_t abort;
+  uint32_t pad;
+  uint64_t ns;
+};
+// Wait for a phase, at most the limit and until another role of the CTA has given
 // up. Each try may sleep up to the hint (100 us) and wakes when the phase ends:
 // warps that poll take issue slots and shared-memory accesses from the others.
+// The result is the thread's own: a phase can end, or a role give up, between two
+// lanes' tries. A warp that goes on together takes __all_sync of it.
 __device__ __forceinline__ bool pair_try_wait(uint64_t *bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(kTryNs)
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort) {
+__device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volatile PairBounds *bounds) {
   if (pair_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
   for (;;) {
     for (int i = 0; i < 32; i++)
       if (pair_try_wait(bar, parity)) return true;
-    if (*abort) return false;
-    if (globaltimer() - t0 > kWaitNs) {
-      *abort = 1;
+    if (bounds->abort) return false;
+    if (globaltimer() - t0 > bounds->ns) {
+      bounds->abort = 1;
       return false;
     }
   }
@@ -235,13 +245,13 @@ struct PairSumsOf {
   static constexpr uint32_t WIDTH = 512 / ACCS;   // columns of an accumulator
   uint64_t *full;
   uint32_t empty_leader;     // cluster address of the leader's empty[0]
-  volatile uint32_t *abort;
+  volatile PairBounds *bounds;
   uint32_t tmem;
   uint32_t n;
   bool ok;
   // Tensor memory address of the next accumulator's columns for this warp's lanes.
   __device__ __forceinline__ uint32_t acquire() {
-    if (ok) ok = __all_sync(0xffffffffu, pair_wait(full + n % ACCS, (n / ACCS) & 1, abort));
+    if (ok) ok = __all_sync(0xffffffffu, pair_wait(full + n % ACCS, (n / ACCS) & 1, bounds));
     tc_fence_after();
     return tmem + (n % ACCS) * WIDTH;
   }
@@ -327,12 +337,12 @@ struct PairNoHelpers {
   static __device__ __forceinline__ void init(uint8_t *) {}
   template <class Args>
   static __device__ __forceinline__ void help(const Args &, uint8_t *, uint32_t, uint32_t, uint32_t,
-                                              volatile uint32_t *) {}
+                                              volatile PairBounds *) {}
 };
 
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    pair_gemm(const __grid_constant__ typename Op::Args args) {
+    pair_gemm(const __grid_constant__ typename Op::Args args, const uint64_t wait_ns) {
   using Shape = PairShape<Op>;
   constexpr int PLANES = Op::PLANES;
   constexpr int KE = Op::KIND == PAIR_E4M3 ? 128 : 64;   // K elements of a block
@@ -348,9 +358,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t *tfull = empty + MAXS;
   uint64_t *tempty = tfull + ACCS;
   uint64_t *drain = tempty + ACCS;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-  volatile uint32_t *abort = tmem_slot + 1;
-  static_assert((2 * MAXS + 2 * ACCS + 1) * 8 + 8 <= Shape::BAR_BYTES, "barriers");
+  PairBounds *bounds = reinterpret_cast<PairBounds *>(drain + 1);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bounds + 1);
+  static_assert((2 * MAXS + 2 * ACCS + 1) * 8 + sizeof(PairBounds) + 4 <= Shape::BAR_BYTES, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
@@ -367,7 +377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       mbar_init(tempty + b, 2 * kPairEpi);
     }
     mbar_init(drain, 1);
-    *abort = 0;
+    *bounds = {0u, 0u, wait_ns};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kPairEpi + 1) {
@@ -386,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   if (warp < kPairEpi) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpiRegs));
-    PairSumsOf<ACCS> sums{tfull, map_to_leader(smem_u32(tempty)), abort, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
+    PairSumsOf<ACCS> sums{tfull, map_to_leader(smem_u32(tempty)), bounds, tmem + (((uint32_t)warp & 3u) << 21), 0u, true};
     Op::epilogue(args, sums, scratch, rank, cluster, clusters);
     BoxStore::finish();
   } else {
@@ -394,12 +404,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (warp == kPairEpi) {
       if (lane == 0) {
         uint32_t s = 0, round = 0;
-        bool ok = true;
+        // (a limit below one try's sleep could not run out while loads come in: it stands for loads that never do)
+        bool ok = wait_ns >= kTryNs;
         for (uint32_t i = cluster; i < items && ok; i += clusters) {
           const PairItem w = Op::item(args, i);
           const int32_t ar = w.a_row + (Op::A_SAME ? 0 : (int32_t)rank * 128), br = w.b_row + (int32_t)(rank * (args.bn / 2));
           for (uint32_t kb = 0; kb < w.kblocks; kb++) {
-            if (!pair_wait(empty + s, (round & 1) ^ 1, abort)) {
+            if (!pair_wait(empty + s, (round & 1) ^ 1, bounds)) {
               ok = false;
               break;
             }
@@ -441,11 +452,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           for (uint32_t kb = 0; kb < w.kblocks; kb++) {
             const bool first = Op::CHUNK ? kb % (Op::CHUNK + !Op::CHUNK) == 0 : kb == 0;
             const bool last = kb + 1 == w.kblocks || (Op::CHUNK && (kb + 1) % (Op::CHUNK + !Op::CHUNK) == 0);
-            if (first && !pair_wait(tempty + acc % ACCS, ((acc / ACCS) & 1) ^ 1, abort)) {
+            if (first && !pair_wait(tempty + acc % ACCS, ((acc / ACCS) & 1) ^ 1, bounds)) {
               ok = false;
               break;
             }
-            if (!pair_wait(full + s, round & 1, abort)) {
+            if (!pair_wait(full + s, round & 1, bounds)) {
               ok = false;
               break;
             }
@@ -485,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         uint64_t t0 = globaltimer();
         while (!mbar_try_wait(drain, 0) && globaltimer() - t0 < kWaitNs) {
         }
-        if (*abort) {
+        if (*static_cast<volatile uint32_t *>(&bounds->abort)) {
           t0 = globaltimer();
           for (uint32_t s = 0; s < stages; s++)
             for (uint32_t parity = 0; parity < 2; parity++)
@@ -495,7 +506,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       __syncwarp();
     } else if (Op::HELPERS) {
-      Op::help(args, scratch, rank, cluster, clusters, abort);
+      Op::help(args, scratch, rank, cluster, clusters, bounds);
     }
   }
   tc_fence_before();
@@ -524,7 +535,7 @@ cudaError_t launch_pair(const typename Op::Args &args, uint32_t items, int sms, 
     set.fetch_or(bit, std::memory_order_relaxed);
   }
   const uint32_t clusters = items < (uint32_t)(sms / 2) ? items : (uint32_t)(sms / 2);
-  return launch_chained(after, pair_gemm<Op>, 2 * clusters, kPairThreads, smem, st, args);
+  return launch_chained(after, pair_gemm<Op>, 2 * clusters, kPairThreads, smem, st, args, pipeline_wait_ns());
 }
 
 }  // namespace annb200

@@ -1360,10 +1360,11 @@ uint32_t prefetch_tiles() {
   return n;
 }
 
-// The limit of each pipeline wait in the flat tensor scan: 4 s, or, for
-// tests of the time-out path, ANN_B200_PIPELINE_WAIT_NS (read at every
-// launch). A wait that runs out sets FLAG_TIMEOUT and the search fails with
-// ANN_BACKEND_ERROR; the drains that follow keep their 4 s.
+// The limit of each pipeline wait in the flat tensor scan and the operators'
+// pair products: 4 s, or, for tests of the time-out path,
+// ANN_B200_PIPELINE_WAIT_NS (read at every launch). A wait that runs out sets
+// FLAG_TIMEOUT and the search fails with ANN_BACKEND_ERROR (an operator's
+// outputs are NaN); the drains that follow keep their 4 s.
 uint64_t pipeline_wait_ns() {
   const char *v = getenv("ANN_B200_PIPELINE_WAIT_NS");
   if (v && *v) {
