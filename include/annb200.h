@@ -604,8 +604,12 @@ int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
  * dense in dtype, overwritten, apart from every input; either may be NULL.
  * The logits are computed
  * again, piece by piece. Each piece of G is held in 16 bits for FP16 and BF16
- * operands, two FP16 terms for FP32 operands. Results do not depend on timing: no
- * atomics. A non-finite value makes non-finite what the formulas make so.
+ * operands, two FP16 terms for FP32 operands; FP16 terms hold G_ij to within
+ * 2^-39 |grad_i| at best, so what falls below that counts as 0, whatever the
+ * other queries' weights are. In drows, grad_i query_i is held to within 2^-38
+ * of the largest |grad| times the largest |value| of a query. Results do not
+ * depend on timing: no atomics. A non-finite value makes non-finite what the
+ * formulas make so.
  *
  * Both calls only enqueue work on stream, on the current device, can be
  * captured into a graph, and use workspace (device, 256-byte aligned, at

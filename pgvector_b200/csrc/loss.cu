@@ -51,11 +51,19 @@ __device__ __forceinline__ float undo_scale(uint32_t bits) {
   const int e = min(120, max(-120, 14 - ((int)(bits >> 23) - 127)));
   return __uint_as_float((uint32_t)(127 - e) << 23);
 }
-// The power of two that grad is divided by: at most its largest |value|.
-__device__ __forceinline__ float grad_unit(uint32_t bits) {
+// G in FP16 terms: FP16 holds 2^-24 to 2^16, so a query's row of G is kept as
+// grad / unit * 2^14 * (p - onehot), below 2^15, where unit is its own |grad|'s
+// power of two: what p falls to is then held to within 2^-39 of 1 whatever the
+// other queries' weights are (with one unit for all, a weight of 2e-7 of the
+// largest lost most of dX over 100,003 rows). dX's factor is
+// a query's, so it undoes the unit; dW sums over queries, and is made with rows
+// x_i * unit_i / (the largest unit), laid out a second time, where 2^-39 of the
+// largest weight's share is all that is lost. BF16 has FP32's range: no unit.
+constexpr float kGradScale = 16384.0f;
+template <typename O> constexpr bool kGradUnits = std::is_same<O, __half>::value;
+__device__ __forceinline__ float grad_unit(uint32_t bits) {   // of |grad|'s bits
   return __uint_as_float(max(bits & 0x7f800000u, 0x00800000u));
 }
-constexpr float kGradScale = 16384.0f;   // G is kept as grad / unit * 2^14 * (p - onehot): below 2^15
 
 __device__ __forceinline__ bool has_target(int64_t t, uint64_t nrows) { return t >= 0 && t < (int64_t)nrows; }
 
@@ -84,7 +92,7 @@ __device__ __forceinline__ uint32_t join_parts(const uint32_t *parts, int n) {
   for (int i = threadIdx.x; i < n; i += 256) best = max(best, parts[i]);
   return block_max(best);
 }
-// The gradient's unit (a warp's lanes together).
+// The largest query's unit (a warp's lanes together).
 __device__ __forceinline__ float grad_unit(const Maxima *m) {
   static_assert(kGradParts == 32, "a part a lane");
   return grad_unit(__reduce_max_sync(0xffffffffu, m->grad[threadIdx.x & 31]));
@@ -95,52 +103,72 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return b < 0x7f800000u ? b : 0u;
 }
 
-// FP32: the largest finite |x| of the rows and, in the gradient, of the queries
-// with a target. `tx` threads a row, 4 values each.
-__global__ void __launch_bounds__(256) find_maxima(const float *w, uint64_t w_stride, uint64_t nrows, const float *x,
-                                                   uint64_t x_stride, uint32_t nq, uint32_t dims, uint32_t tx,
-                                                   const int64_t *targets, Maxima *out) {
+// The largest finite |x| of the rows (FP32), of the queries with a target, and
+// of those queries' weights: kRowParts, kQueryParts and kGradParts blocks, where
+// they are asked for. `tx` threads a row, 16 bytes each.
+template <typename T> struct FindMaxima {
+  const T *w, *x;
+  uint64_t w_stride, x_stride, nrows;
+  uint32_t nq, dims, tx;
+  uint32_t row_blocks, query_blocks, grad_blocks;
+  const int64_t *targets;
+  const float *grad;
+  Maxima *out;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) find_maxima(const FindMaxima<T> p) {
+  constexpr uint32_t V = 16 / sizeof(T);
   chain_next();
-  const bool queries = blockIdx.x >= kRowParts;
-  const uint32_t block = queries ? blockIdx.x - kRowParts : blockIdx.x, grid = queries ? kQueryParts : kRowParts;
-  const float *from = queries ? x : w;
-  const uint64_t stride = queries ? x_stride : w_stride, rows = queries ? nq : nrows;
-  const uint32_t cx = threadIdx.x % tx, ry = threadIdx.x / tx, ty = 256 / tx;
-  const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+  const bool queries = blockIdx.x >= p.row_blocks;
+  const uint32_t block = queries ? blockIdx.x - p.row_blocks : blockIdx.x, grid = queries ? p.query_blocks : p.row_blocks;
   uint32_t best = 0;
+  if (queries && block >= p.query_blocks) {
+    for (uint32_t q = (block - p.query_blocks) * 256 + threadIdx.x; q < p.nq; q += p.grad_blocks * 256)
+      if (has_target(p.targets[q], p.nrows)) best = max(best, finite_bits(p.grad[q]));
+    best = block_max(best);
+    if (threadIdx.x == 0) p.out->grad[block - p.query_blocks] = best;
+    return;
+  }
+  const T *from = queries ? p.x : p.w;
+  const uint64_t stride = queries ? p.x_stride : p.w_stride, rows = queries ? p.nq : p.nrows;
+  const uint32_t cx = threadIdx.x % p.tx, ry = threadIdx.x / p.tx, ty = 256 / p.tx;
+  const bool vec = stride % V == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
   for (uint64_t r = (uint64_t)block * ty + ry; r < rows; r += (uint64_t)grid * ty) {
-    if (queries && !has_target(targets[r], nrows)) continue;
-    const float *row = from + r * stride;
-    for (uint32_t c = cx * 4; c < dims; c += tx * 4) {
-      if (vec && c + 4 <= dims) {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(row + c));
-        best = max(max(best, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+    if (queries && !has_target(p.targets[r], p.nrows)) continue;
+    const T *row = from + r * stride;
+    for (uint32_t c = cx * V; c < p.dims; c += p.tx * V) {
+      if (vec && c + V <= p.dims) {
+        alignas(16) T v[V];
+        *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(row + c));
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) best = max(best, finite_bits(to_float(v[j])));
       } else {
-        for (uint32_t j = c; j < min(dims, c + 4); j++) best = max(best, finite_bits(row[j]));
+        for (uint32_t j = c; j < min(p.dims, c + V); j++) best = max(best, finite_bits(to_float(row[j])));
       }
     }
   }
   best = block_max(best);
-  if (threadIdx.x == 0) (queries ? out->queries : out->rows)[block] = best;
+  if (threadIdx.x == 0) (queries ? p.out->queries : p.out->rows)[block] = best;
 }
 
 // Operands in the layout TMA reads: `ld` values (a multiple of 8) a row, values
 // past dims zero. FP32: two FP16 planes of x * 2^e; an infinity becomes NaN (its
-// products with a low term of 0 would be).
+// products with a low term of 0 would be). weighted: dW's queries, x * 2^e * unit /
+// the largest unit (kGradScale); of FP16 operands too, with the e of all queries.
 template <typename T, typename O, int PLANES> struct Layout {
   const T *x, *w;
   uint64_t x_stride, w_stride, nrows;
   uint32_t nq, dims, ld;
   uint32_t tx;                     // threads a row of w, 8 values each
-  uint32_t query_blocks, row_blocks, grad_blocks;
+  uint32_t query_blocks, row_blocks;
   const int64_t *targets;
   const float *grad;
   bool leave_out;                  // the gradient's: queries without a target become rows of zeros, one e for all
-  O *xo, *wo;
+  O *xo, *wo, *weighted;
   float *xscale;                   // PLANES 2: 2^-e of each query
   Maxima *maxima;
 };
-template <typename T, typename O, int PLANES>
+template <typename T, typename O, int PLANES, bool MUL = PLANES == 2>
 __device__ __forceinline__ void pack8(const T *row, uint32_t c, uint32_t dims, bool vec, bool zero, float mul, O *out,
                                       uint64_t plane) {
   alignas(16) T v[8];
@@ -153,6 +181,10 @@ __device__ __forceinline__ void pack8(const T *row, uint32_t c, uint32_t dims, b
     for (int j = 0; j < 8; j++) v[j] = !zero && c + j < dims ? row[c + j] : from_float<T>(0.0f);
   }
   if constexpr (PLANES == 1) {
+    if constexpr (MUL) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = from_float<T>(to_float(v[j]) * mul);
+    }
     *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<uint4 *>(v);
   } else {
     uint32_t hi[4], lo[4];
@@ -183,10 +215,12 @@ __global__ void __launch_bounds__(256) lay_out(const Layout<T, O, PLANES> p) {
     const uint32_t lane = threadIdx.x % 32;
     const bool vec = p.x_stride % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0;
     uint32_t all = 0;
-    if (PLANES == 2 && p.leave_out) {
+    if ((PLANES == 2 && p.leave_out) || (kGradUnits<O> && p.weighted)) {
       all = join_parts(p.maxima->queries, kQueryParts);
       if (block == 0 && threadIdx.x == 0) p.maxima->all_queries = all;
     }
+    float largest = 1.0f;
+    if (kGradUnits<O> && p.weighted) largest = grad_unit(p.maxima);
     const uint32_t q = block * 8 + threadIdx.x / 32;
     if (q >= p.nq) return;
     const T *row = p.x + q * p.x_stride;
@@ -199,6 +233,20 @@ __global__ void __launch_bounds__(256) lay_out(const Layout<T, O, PLANES> p) {
     for (uint32_t c = lane * 8; c < p.ld; c += 256)
       pack8<T, O, PLANES>(row, c, p.dims, vec, zero, mul, p.xo + (uint64_t)q * p.ld + c, (uint64_t)p.nq * p.ld);
     if (PLANES == 2 && lane == 0) p.xscale[q] = undo;
+    if constexpr (kGradUnits<O>) {
+      if (p.weighted) {
+        // 2^e unit / largest as an exponent, from -126 on (a weight that is not finite, or not a query's with a
+        // target, is none of those that the largest is taken from)
+        const uint32_t w = __float_as_uint(p.grad[q]) & 0x7fffffffu;
+        const float unit = !zero && w < 0x7f800000u ? grad_unit(w) : largest;
+        const int up = (int)(__float_as_uint(mul) >> 23) + (int)(__float_as_uint(unit) >> 23) -
+                       (int)(__float_as_uint(largest) >> 23);
+        const float m = __uint_as_float((uint32_t)max(up, 1) << 23);
+        for (uint32_t c = lane * 8; c < p.ld; c += 256)
+          pack8<T, O, PLANES, true>(row, c, p.dims, vec, zero, m, p.weighted + (uint64_t)q * p.ld + c,
+                                    (uint64_t)p.nq * p.ld);
+      }
+    }
     return;
   }
   block -= p.query_blocks;
@@ -214,14 +262,7 @@ __global__ void __launch_bounds__(256) lay_out(const Layout<T, O, PLANES> p) {
     for (uint64_t r = (uint64_t)block * ty + ry; r < p.nrows; r += (uint64_t)p.row_blocks * ty)
       for (uint32_t c = cx * 8; c < p.ld; c += p.tx * 8)
         pack8<T, O, PLANES>(p.w + r * p.w_stride, c, p.dims, vec, false, mul, p.wo + r * p.ld + c, p.nrows * p.ld);
-    return;
   }
-  block -= p.row_blocks;
-  uint32_t best = 0;
-  for (uint32_t q = block * 256 + threadIdx.x; q < p.nq; q += p.grad_blocks * 256)
-    if (has_target(p.targets[q], p.nrows)) best = max(best, p.grad ? finite_bits(p.grad[q]) : 0x3f800000u);
-  best = block_max(best);
-  if (threadIdx.x == 0) p.maxima->grad[block] = best;
 }
 
 // ---------------------------------------------------------------- logits
@@ -303,7 +344,6 @@ struct LogitsOp : PairNoHelpers {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t share = (FEW ? 2 * rank : 0) + (warp >> 2);   // which columns of a tile
     const double scale2 = PLANES == 2 ? p.scale2 * (double)undo_scale(p.maxima->all_rows) : p.scale2;
-    const float unit = GRAD ? grad_unit(p.maxima) : 1.0f;
     BoxStore box{scratch + 2 * warp * kBoxBytes};
     uint32_t turn = 0;
     Row next = row_of(p, cluster, rank);
@@ -387,7 +427,9 @@ struct LogitsOp : PairNoHelpers {
         // p = exp2(l2 - lse2) c: c is what rounding lse2 (the lse in base 2) lost
         const float lse2 = row.lse * kLog2e;
         const float c = exp2f(-(fmaf(row.lse, kLog2e, -lse2) + row.lse * kLog2eLow));
-        const float g = kept ? row.grad / unit * kGradScale * c : 0.0f, one = 1.0f / c;
+        const float held = kGradUnits<O> ? row.grad / grad_unit(__float_as_uint(row.grad) & 0x7fffffffu) * kGradScale
+                                         : row.grad;
+        const float g = kept ? held * c : 0.0f, one = 1.0f / c;
         const f32x2 kk = pack2(k, k), zz = pack2(-lse2, -lse2), gg = pack2(g, g);
 #pragma unroll
         for (int j = 0; j < COLS / 2; j++) {
@@ -553,18 +595,19 @@ struct QueriesOp : PairNoHelpers {
 };
 
 // dW: 256 of the piece's rows x bn dimensions, K = the queries.
-template <PairKind KIND_, int PLANES_, typename T>
+template <PairKind KIND_, int PLANES_, typename T, typename O>
 struct RowsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = true, B_MN = true;
   static constexpr int PLANES = PLANES_, SCRATCH = kPairEpi * kBoxBytes, MAX_STAGES = 8;
   static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
   struct Args {
-    CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); X
+    CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); X, weighted where the queries have weights
     uint32_t bn;
     uint32_t mt, nt, kblocks;
     uint32_t rows, dims;     // rows of the piece
     double scale;
+    bool weighted;
     const Maxima *maxima;
     T *out;                  // the piece's first row
     int boxes;               // out's rows are 16-byte aligned: `map` stores them
@@ -582,8 +625,12 @@ struct RowsOp : PairNoHelpers {
                                               uint32_t rank) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const uint32_t i = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
-    double f = p.scale * (double)grad_unit(p.maxima) / kGradScale;
-    if (PLANES == 2) f *= (double)undo_scale(p.maxima->all_queries);
+    double f = p.scale;
+    if (kGradUnits<O>) {
+      f /= kGradScale;
+      if (p.weighted) f *= (double)grad_unit(p.maxima);
+      if (PLANES == 2 || p.weighted) f *= (double)undo_scale(p.maxima->all_queries);
+    }
     const float factor = (float)f;
     const uint32_t cols = p.bn / 2;
     f32x2 v[64];
@@ -635,9 +682,9 @@ struct RowsOp : PairNoHelpers {
 // whole row (10 times G's rounding where a cluster's rows differ by a tenth of
 // their length). With it taken off at the target, the sum is over
 // G_ij (w_j - w_target), and errors are relative to the differences.
-template <typename T, int PLANES>
+template <typename T, typename O, int PLANES>
 __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t splits, uint32_t nq, uint32_t dims,
-                                                    double scale, const Maxima *maxima, const float *gsum,
+                                                    double scale, const float *grad, const Maxima *maxima, const float *gsum,
                                                     uint32_t gsums, const T *rows, uint64_t stride,
                                                     const int64_t *targets, uint64_t nrows, T *out) {
   chain_wait();
@@ -649,8 +696,11 @@ __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t 
     for (uint32_t d = threadIdx.x; d < dims; d += 256) to[d] = from_float<T>(0.0f);
     return;
   }
-  const float factor = (float)(scale * (double)grad_unit(maxima) / kGradScale);
-  const float undo = PLANES == 2 ? undo_scale(maxima->all_rows) : 1.0f;
+  double f = scale;
+  if (kGradUnits<O>) f *= (double)(grad ? grad_unit(__float_as_uint(grad[q]) & 0x7fffffffu) : 1.0f) / kGradScale;
+  // the partial sums are in units of the rows' undo: the target's row is brought there, powers of two
+  const float undo = PLANES == 2 ? undo_scale(maxima->all_rows) : 1.0f, up = 1.0f / undo;
+  const float factor = (float)(f * (double)undo);
   const T *row = rows + (uint64_t)t * stride;
   const float *at = part + (uint64_t)q * ld;
   constexpr uint32_t EACH = 4;     // dimensions a thread: loaded before the sum of G is waited for
@@ -662,7 +712,7 @@ __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t 
       v[u] = 0.0f;
       r[u] = 0.0f;
       if (d < dims) {
-        r[u] = to_float(row[d]);
+        r[u] = to_float(row[d]) * up;
         for (uint32_t k = 0; k < splits; k++) v[u] += at[k * plane + d];
       }
     }
@@ -683,7 +733,7 @@ __global__ void __launch_bounds__(256) join_queries(const float *part, uint32_t 
 #pragma unroll
     for (uint32_t u = 0; u < EACH; u++) {
       const uint32_t d = d0 + threadIdx.x + 256 * u;
-      if (d < dims) to[d] = from_float<T>(fmaf(left, r[u], v[u] * undo) * factor);
+      if (d < dims) to[d] = from_float<T>(fmaf(left, r[u], v[u]) * factor);
     }
   }
 }
@@ -710,7 +760,8 @@ struct Plan {
   int planes;
   uint32_t ld;             // values a packed row
   bool pack_x, pack_w;
-  uint64_t x, w, xscale, maxima, part, tlogit, g, gsum, dq, total;
+  bool weighted;           // dW's queries are laid out apart (kGradScale)
+  uint64_t x, w, xw, xscale, maxima, part, tlogit, g, gsum, dq, total;
   bool few;                // up to 128 queries (LogitsOp)
   uint32_t parts;          // partial sums a tile
   uint32_t nt, chunk;      // row tiles; forward: queries a launch
@@ -730,6 +781,8 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
   p.xscale = c.take(nq * 4);
   if (p.pack_x) p.x = c.take(nq * p.ld * 2 * p.planes);
   if (p.pack_w) p.w = c.take(j.nrows * p.ld * 2 * p.planes);
+  p.weighted = grad && j.grad && j.dtype != ANNB200_BF16;
+  if (p.weighted) p.xw = c.take(nq * p.ld * 2 * p.planes);
   p.nt = (uint32_t)((j.nrows + 255) / 256);
   p.few = nq <= 128;
   p.parts = p.few ? 4 : 2;
@@ -811,16 +864,29 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     wo = lay.wo = reinterpret_cast<O *>(ws + p.w);
     wld = p.ld;
   }
-  if (grad) lay.grad_blocks = kGradParts;
-  if (PLANES == 2) {
-    uint32_t tx = 1;
-    while (tx < 256 && tx * 4 < j.dims) tx *= 2;
-    find_maxima<<<kRowParts + (grad ? kQueryParts : 0), 256, 0, st>>>(
-        reinterpret_cast<const float *>(w), j.row_stride, j.nrows, reinterpret_cast<const float *>(x), j.query_stride,
-        j.nq, j.dims, tx, j.targets, maxima);
+  const bool weighted = p.weighted && j.drows;
+  if (weighted) lay.weighted = reinterpret_cast<O *>(ws + p.xw);
+  if (PLANES == 2 || weighted) {
+    FindMaxima<T> find = {};
+    find.w = w;
+    find.x = x;
+    find.w_stride = j.row_stride;
+    find.x_stride = j.query_stride;
+    find.nrows = j.nrows;
+    find.nq = j.nq;
+    find.dims = j.dims;
+    find.tx = 1;
+    while (find.tx < 256 && find.tx * (16 / sizeof(T)) < j.dims) find.tx *= 2;
+    find.row_blocks = PLANES == 2 ? kRowParts : 0;
+    find.query_blocks = grad ? kQueryParts : 0;
+    find.grad_blocks = weighted ? kGradParts : 0;
+    find.targets = j.targets;
+    find.grad = j.grad;
+    find.out = maxima;
+    find_maxima<<<find.row_blocks + find.query_blocks + find.grad_blocks, 256, 0, st>>>(find);
     launches++;
   }
-  if (const uint32_t blocks = lay.query_blocks + lay.row_blocks + lay.grad_blocks) {
+  if (const uint32_t blocks = lay.query_blocks + lay.row_blocks) {
     e = launch_chained(launches > 0, lay_out<T, O, PLANES>, blocks, 256, 0, st, lay);
     launches++;
     if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss: %s", cudaGetErrorString(e));
@@ -873,7 +939,7 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
   const uint64_t gplane = (uint64_t)j.nq * p.piece;
   using LOp = LogitsOp<KIND, PLANES, true, FEW, O>;
   using QOp = QueriesOp<KIND, PLANES>;
-  using ROp = RowsOp<KIND, PLANES, T>;
+  using ROp = RowsOp<KIND, PLANES, T, O>;
   typename LOp::Args l = {};
   logits(l);
   l.mt = (j.nq + 255) / 256;
@@ -907,7 +973,8 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     if (j.drows && e == cudaSuccess) {
       typename ROp::Args a = {};
       map(a.a, g, n, j.nq, p.piece, gplane, 64);
-      map(a.b, xo, j.dims, j.nq, xld, (uint64_t)j.nq * p.ld, 64);
+      map(a.b, weighted ? lay.weighted : xo, j.dims, j.nq, xld, (uint64_t)j.nq * p.ld, 64);
+      a.weighted = weighted;
       a.bn = p.bn;
       a.mt = (uint32_t)((n + 255) / 256);
       a.nt = p.dt;
@@ -926,8 +993,8 @@ int run_loss(const AnnB200LossJob &j, bool grad, cudaStream_t st) {
     }
   }
   if (j.dqueries && e == cudaSuccess) {
-    e = launch_chained(true, join_queries<T, PLANES>, j.nq, 256, 0, st, dq, p.splits, j.nq, j.dims, (double)j.scale,
-                       maxima, l.gsum, l.gsums, w, j.row_stride, j.targets, j.nrows, static_cast<T *>(j.dqueries));
+    e = launch_chained(true, join_queries<T, O, PLANES>, j.nq, 256, 0, st, dq, p.splits, j.nq, j.dims, (double)j.scale,
+                       j.grad, maxima, l.gsum, l.gsums, w, j.row_stride, j.targets, j.nrows, static_cast<T *>(j.dqueries));
     launches++;
   }
   if (e != cudaSuccess) return report_error(OP_BACKEND_ERROR, "softmax loss gradient: %s", cudaGetErrorString(e));
