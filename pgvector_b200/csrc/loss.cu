@@ -537,7 +537,7 @@ struct QueriesOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = false, B_MN = true;
   static constexpr int PLANES = PLANES_, SCRATCH = kPairEpi * kBoxBytes, MAX_STAGES = 8;
-  static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
+  static constexpr int CHUNK = PLANES == 2 ? 2 : 64;   // 24 or 256 steps of the tensor cores
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); W's rows from the piece's first on
     uint32_t bn;
@@ -565,32 +565,25 @@ struct QueriesOp : PairNoHelpers {
     const uint32_t q = (uint32_t)w.a_row + rank * 128 + (warp & 3) * 32 + lane;
     const uint32_t cols = p.bn / 2;
     f32x2 v[64];
-    uint32_t tmem = 0;
-    if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
-    else tmem = sums.acquire() + half * cols;
+    sums.template total<CHUNK, 4>(half * cols, w.kblocks, v);
     BoxStore box{scratch + warp * kBoxBytes};
 #pragma unroll
     for (uint32_t c = 0; c < 4; c++) {
       const uint32_t d0 = (uint32_t)w.b_row + half * cols + c * 32;
       if (c * 32 >= cols || d0 >= p.dims || q - lane >= p.nq) break;
       uint32_t r[32];
-      if (CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-          float a, b;
-          unpack2(v[16 * c + j], a, b);
-          r[2 * j] = __float_as_uint(a);
-          r[2 * j + 1] = __float_as_uint(b);
-        }
-      } else {
-        sums.load(tmem + c * 32, r);
+      for (int j = 0; j < 16; j++) {
+        float a, b;
+        unpack2(v[16 * c + j], a, b);
+        r[2 * j] = __float_as_uint(a);
+        r[2 * j + 1] = __float_as_uint(b);
       }
       box.reuse();
 #pragma unroll
       for (int j = 0; j < 8; j++) box.put(j, make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]));
       box.store_sums(&p.part, (int32_t)d0, (int32_t)(q - lane), (int32_t)w.index, p.add != 0);
     }
-    if (!CHUNK) sums.release();
   }
 };
 
@@ -600,7 +593,7 @@ struct RowsOp : PairNoHelpers {
   static constexpr PairKind KIND = KIND_;
   static constexpr bool A_MN = true, B_MN = true;
   static constexpr int PLANES = PLANES_, SCRATCH = kPairEpi * kBoxBytes, MAX_STAGES = 8;
-  static constexpr int CHUNK = PLANES == 2 ? 2 : 0;
+  static constexpr int CHUNK = PLANES == 2 ? 2 : 64;   // 24 or 256 steps of the tensor cores
   struct Args {
     CUtensorMap a[PLANES], b[PLANES];   // G (piece columns); X, weighted where the queries have weights
     uint32_t bn;
@@ -634,9 +627,7 @@ struct RowsOp : PairNoHelpers {
     const float factor = (float)f;
     const uint32_t cols = p.bn / 2;
     f32x2 v[64];
-    uint32_t tmem = 0;
-    if (CHUNK) sums.template total<CHUNK + !CHUNK, 4>(half * cols, w.kblocks, v);
-    else tmem = sums.acquire() + half * cols;
+    sums.template total<CHUNK, 4>(half * cols, w.kblocks, v);
     BoxStore box{scratch + warp * kBoxBytes};
     constexpr uint32_t BOX = 128 / sizeof(T), V = 16 / sizeof(T);   // values of a box row, of a chunk
 #pragma unroll
@@ -644,16 +635,12 @@ struct RowsOp : PairNoHelpers {
       const uint32_t d0 = (uint32_t)w.b_row + half * cols + c * 32;
       if (c * 32 >= cols || d0 >= p.dims || i - lane >= p.rows) break;
       uint32_t r[32];
-      if (CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-          float a, b;
-          unpack2(v[16 * c + j], a, b);
-          r[2 * j] = __float_as_uint(a);
-          r[2 * j + 1] = __float_as_uint(b);
-        }
-      } else {
-        sums.load(tmem + c * 32, r);
+      for (int j = 0; j < 16; j++) {
+        float a, b;
+        unpack2(v[16 * c + j], a, b);
+        r[2 * j] = __float_as_uint(a);
+        r[2 * j + 1] = __float_as_uint(b);
       }
       const uint32_t at = c * 32 % BOX;     // of the box's values
       if (at == 0) box.reuse();
@@ -671,7 +658,6 @@ struct RowsOp : PairNoHelpers {
         else box.copy(p.out + (uint64_t)y * p.dims + x, p.dims, min(32u, p.rows - y), min(BOX, p.dims - x));
       }
     }
-    if (!CHUNK) sums.release();
   }
 };
 
