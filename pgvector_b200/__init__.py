@@ -27,6 +27,7 @@ import numpy as np
 
 from . import _abi
 from ._lib import (OK, INVALID, UNSUPPORTED, NOMEM, BACKEND_ERROR, AnnB200Error, check, load)
+from .ops import matmul_blocks, quantize_blocks, softmax_loss, softmax_loss_grad
 
 F32, F16, E4M3, NVFP4, BIT, BF16 = 0, 1, 2, 3, 4, 5
 L2, IP, COSINE, HAMMING = 0, 1, 2, 3
@@ -348,18 +349,6 @@ def search_typed(jobs):
                                     for q in range(nq)]))
     del keep
     return out
-
-
-_OPS = ('softmax_loss', 'softmax_loss_grad', 'quantize_blocks', 'matmul_blocks')
-
-
-def __getattr__(name):
-    """The operators, on first use: ops.py needs torch, the rest only where it is called."""
-    if name in _OPS:
-        from . import ops
-        globals().update({n: getattr(ops, n) for n in _OPS})
-        return globals()[name]
-    raise AttributeError('module %r has no attribute %r' % (__name__, name))
 
 
 __all__ = ['softmax_loss', 'softmax_loss_grad', 'quantize_blocks', 'matmul_blocks', 'BF16',

@@ -14,14 +14,22 @@ arguments raise AnnB200Error (ANN_INVALID).
 import contextlib
 import ctypes
 
-import torch
-
 from . import _abi
 from ._lib import AnnB200Error, INVALID, check, load
 
 BLOCK = 128
-TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 5}
-E4M3 = (torch.float8_e4m3fn, torch.uint8)
+# torch, its types' numbers in annb200.h and those of E4M3 codes: from the first
+# call on (the package and its names are there without torch)
+torch, TYPES, E4M3 = None, {}, ()
+
+
+def _with_torch():
+    global torch, TYPES, E4M3
+    if torch is None:
+        import torch as module
+        TYPES = {module.float32: 0, module.float16: 1, module.bfloat16: 5}
+        E4M3 = (module.float8_e4m3fn, module.uint8)
+        torch = module
 
 
 def _need(ok, message, *args):
@@ -104,6 +112,7 @@ def softmax_loss(queries, rows, targets, scale=1.0, status=None, stream=None):
     (float32, float16, bfloat16); targets int64 [nq], negative for none (loss
     0). status: optional int32 [nq], ANN_INVALID for a target >= n (loss NaN).
     Returns (loss, lse), float32 [nq]."""
+    _with_torch()
     job = _loss_job(queries, rows, targets, scale)
     nq, device = queries.shape[0], rows.device
     if status is not None:
@@ -127,6 +136,7 @@ def softmax_loss_grad(queries, rows, targets, lse, grad=None, scale=1.0, need_qu
     default ones. Returns (dqueries, drows) of the operands' type; None for one
     that is not needed. With torch.autograd in the encoder:
     ``queries.backward(dqueries)``."""
+    _with_torch()
     job = _loss_job(queries, rows, targets, scale)
     nq, device = queries.shape[0], rows.device
     job.lse = _vector(lse, 'lse', nq, torch.float32, rows)
@@ -154,6 +164,7 @@ def quantize_blocks(x, square=False, stream=None):
     per 1 x 128 block of a row, or per 128 x 128 block (square). Returns
     (codes float8_e4m3fn [m, k], a view of rows of a multiple of 16 bytes;
     scales float32 [m or ceil(m/128), ceil(k/128)])."""
+    _with_torch()
     stride = _matrix(x, 'x', TYPES)
     m, k = x.shape
     pad = (k + 15) // 16 * 16
@@ -188,6 +199,7 @@ def matmul_blocks(a, a_scales, b, b_scales, dtype=None, stream=None):
     (rows a multiple of 16 bytes apart, 16-byte aligned). Each side's scales
     have one row per row, or one per 128 rows (square blocks). dtype: float32
     (default), float16 or bfloat16. Returns [m, n]."""
+    _with_torch()
     dtype = dtype or torch.float32
     _need(dtype in TYPES, 'output type %s', dtype)
     sa, qa = _operand(a, a_scales, 'a')
