@@ -9,10 +9,13 @@ out; the kernels are libannb200.so's, see annb200.h for the exact terms).
 Calls enqueue their work on ``stream`` (default: torch's current stream of the
 operands' device) and return at once. Their outputs and workspace are
 allocated for that stream, so they can be captured into a CUDA graph. Bad
-arguments raise AnnB200Error (ANN_INVALID).
+arguments raise AnnB200Error (ANN_INVALID). softmax_loss takes part in autograd;
+codes, scales and products of codes are not differentiable and never require a
+gradient.
 """
 import contextlib
 import ctypes
+import functools
 
 from . import _abi
 from ._lib import AnnB200Error, INVALID, check, load
@@ -111,22 +114,58 @@ def softmax_loss(queries, rows, targets, scale=1.0, status=None, stream=None):
     <query_i, row_j>). queries [nq, dims] and rows [n, dims] of one type
     (float32, float16, bfloat16); targets int64 [nq], negative for none (loss
     0). status: optional int32 [nq], ANN_INVALID for a target >= n (loss NaN).
-    Returns (loss, lse), float32 [nq]."""
+    Returns (loss, lse), float32 [nq].
+
+    Where queries or rows require a gradient, so does the loss: its backward pass
+    is softmax_loss_grad, once. lse has no gradient of its own: a backward pass
+    that reaches it raises AnnB200Error. (As with all of torch's operators, a
+    backward pass is captured into a CUDA graph only while no graph of the same
+    leaves made outside of the capture is alive.)"""
     _with_torch()
     job = _loss_job(queries, rows, targets, scale)
-    nq, device = queries.shape[0], rows.device
     if status is not None:
-        job.status = _vector(status, 'status', nq, torch.int32, rows)
+        job.status = _vector(status, 'status', queries.shape[0], torch.int32, rows)
+    if (queries.requires_grad or rows.requires_grad) and torch.is_grad_enabled():
+        return _run(stream, (queries, rows, targets, status),
+                    lambda st: _autograd().apply(queries, rows, targets, job))
+    return _run(stream, (queries, rows, targets, status),
+                lambda st: _enqueue_loss(job, rows.device, st,
+                                         torch.empty((2, job.nq), dtype=torch.float32, device=rows.device).unbind()))
 
-    def call(st):
-        out = torch.empty((2, nq), dtype=torch.float32, device=device)
-        job.loss = out.data_ptr()
-        job.lse = job.loss + 4 * nq if nq else job.loss
-        ws = _workspace(job, 0, device)  # noqa: F841
-        check(load().AnnB200SoftmaxLoss(ctypes.byref(job), st))
-        return out.unbind()
 
-    return _run(stream, (queries, rows, targets, status), call)
+def _enqueue_loss(job, device, st, out):
+    job.loss, job.lse = out[0].data_ptr(), out[1].data_ptr()
+    ws = _workspace(job, 0, device)  # noqa: F841
+    check(load().AnnB200SoftmaxLoss(ctypes.byref(job), st))
+    return out
+
+
+@functools.cache
+def _autograd():
+    class SoftmaxLoss(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, queries, rows, targets, job):
+            # (on the stream that _run made current, and so is the backward pass)
+            loss = torch.empty((job.nq,), dtype=torch.float32, device=rows.device)
+            lse = torch.empty_like(loss)
+            _enqueue_loss(job, rows.device, torch._C._cuda_getCurrentRawStream(rows.device.index), (loss, lse))
+            ctx.save_for_backward(queries, rows, targets, lse)
+            ctx.set_materialize_grads(False)
+            ctx.scale = job.scale
+            return loss, lse
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad, grad_lse):
+            _need(grad_lse is None, 'softmax_loss: lse has no gradient (detach it)')
+            if grad is None:
+                return None, None, None, None
+            queries, rows, targets, lse = ctx.saved_tensors
+            dq, dr = softmax_loss_grad(queries, rows, targets, lse, grad=grad.contiguous(), scale=ctx.scale,
+                                       need_queries=ctx.needs_input_grad[0], need_rows=ctx.needs_input_grad[1])
+            return dq, dr, None, None
+
+    return SoftmaxLoss
 
 
 def softmax_loss_grad(queries, rows, targets, lse, grad=None, scale=1.0, need_queries=True, need_rows=True,
@@ -134,8 +173,8 @@ def softmax_loss_grad(queries, rows, targets, lse, grad=None, scale=1.0, need_qu
     """Gradients of sum_i grad_i * loss_i by the queries and the rows, from the
     inputs of softmax_loss and the lse it returned. grad: float32 [nq], by
     default ones. Returns (dqueries, drows) of the operands' type; None for one
-    that is not needed. With torch.autograd in the encoder:
-    ``queries.backward(dqueries)``."""
+    that is not needed. They are not differentiable further. softmax_loss calls
+    this in its backward pass; by hand, ``queries.backward(dqueries)``."""
     _with_torch()
     job = _loss_job(queries, rows, targets, scale)
     nq, device = queries.shape[0], rows.device

@@ -37,3 +37,16 @@ assert 'torch' not in sys.modules
 import inspect
 assert 'targets' in inspect.signature(softmax_loss).parameters and quantize_blocks.__doc__
 ''')
+
+
+def test_operands_that_need_a_gradient_are_checked_first():
+    run('''
+import torch
+import pgvector_b200 as pb
+x, t = torch.zeros(4, 8, requires_grad=True), torch.zeros(4, dtype=torch.int64)
+try:
+    pb.softmax_loss(x, x, t)
+    raise SystemExit('taken')
+except pb.AnnB200Error as e:
+    assert e.status == pb.INVALID
+''')
