@@ -37,7 +37,7 @@ template <typename T> struct Eight {
 #pragma unroll
       for (int j = 0; j < (int)sizeof(T) / 2; j++) w[j] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + j);
     } else {
-      T t[8];
+      alignas(16) T t[8];   // (read back 16 bytes at a time)
 #pragma unroll
       for (int j = 0; j < 8; j++) t[j] = c + j < k ? row[c + j] : from_float<T>(0.0f);
 #pragma unroll
