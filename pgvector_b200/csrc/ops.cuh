@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/annb200.h"
 #include "internal.cuh"
 
@@ -88,12 +90,12 @@ bool encode_sums_map(CUtensorMap *map, void *base, uint64_t inner, uint64_t oute
 
 // SMs of the current device (a device's number never changes: asked once each).
 inline int op_sms() {
-  static int known[64];
+  static std::atomic<int> known[64];   // (calls come from any thread)
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 0;
-  if (dev < 64 && known[dev]) return known[dev];
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed))) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  if (dev < 64) known[dev] = n;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
