@@ -768,7 +768,7 @@ Plan plan_of(const AnnB200LossJob &j, bool grad) {
   if (p.pack_x) p.x = c.take(nq * p.ld * 2 * p.planes);
   if (p.pack_w) p.w = c.take(j.nrows * p.ld * 2 * p.planes);
   p.weighted = grad && j.grad && j.dtype != ANNB200_BF16;
-  if (p.weighted) p.xw = c.take(nq * p.ld * 2 * p.planes);
+  if (grad && j.dtype != ANNB200_BF16) p.xw = c.take(nq * p.ld * 2 * p.planes);   // (whether or not grad is set yet)
   p.nt = (uint32_t)((j.nrows + 255) / 256);
   p.few = nq <= 128;
   p.parts = p.few ? 4 : 2;
