@@ -117,3 +117,13 @@ def test_weights_times_a_power_of_two(cuda, dtype):
     a, _ = pb.softmax_loss_grad(x, w, t, lse, grad=grad, scale=0.25, need_rows=False)
     _, b = pb.softmax_loss_grad(x, w, t, lse, grad=grad, scale=0.25, need_queries=False)
     assert torch.equal(a, one) and torch.equal(b, rows)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_rows_near_the_largest_values(cuda, dtype):
+    # rows of 2^120: their gradients are in range, and so is what leads to them
+    import torch
+    from test_ops_gpu import check_loss, loss_inputs
+    x, w, t, g = loss_inputs(40, 900, 64, dtype, seed=11)
+    _, _, dx, dw = check_loss(x * 2.0 ** -110, w * 2.0 ** 120, t, g, scale=2.0 ** -8)
+    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dw).all()) and bool(dx.abs().max() > 2.0 ** 105)
