@@ -575,8 +575,10 @@ int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
  *   lse_i  = log sum_j exp(l_ij)
  *   loss_i = lse_i - l_i,target(i)
  *
- * The logits are never kept: like a search, the call walks the rows in
- * pieces and keeps per query only a running maximum and sum, in FP32.
+ * The logits are never kept: of a tile of 256 rows a query leaves two pairs of
+ * a maximum and a sum in FP32 (four, with up to 128 queries) in the workspace,
+ * which a second kernel joins, for as many queries at a time as 256 MB hold
+ * (256 at least).
  *
  * dtype     ANNB200_F32, ANNB200_F16 or ANNB200_BF16: both operands and both
  *           gradients. Products are summed in FP32 (FP32 operands as two
@@ -602,14 +604,18 @@ int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
  *   drows_j    = scale * sum_i G_ij query_i    [nrows][dims]
  *
  * dense in dtype, overwritten, apart from every input; either may be NULL.
- * The logits are computed
- * again, piece by piece. Each piece of G is held in 16 bits for FP16 and BF16
- * operands, two FP16 terms for FP32 operands; FP16 terms hold G_ij to within
- * 2^-39 |grad_i| at best, so what falls below that counts as 0, whatever the
- * other queries' weights are. In drows, grad_i query_i is held to within 2^-38
- * of the largest |grad| times the largest |value| of a query. Results do not
- * depend on timing: no atomics. A non-finite value makes non-finite what the
- * formulas make so.
+ * dqueries is computed as scale * sum_j G_ij (row_j - row_target(i)): the same,
+ * since for the lse of exactly these rows sum_j G_ij = 0. For any other lse (one
+ * joined over several calls' rows, with more terms) it is not: dqueries would be
+ * wrong, and such calls are not supported.
+ *
+ * The logits are computed again, piece by piece. Each piece of G is held in
+ * 16 bits for FP16 and BF16 operands, two FP16 terms for FP32 operands; FP16
+ * terms hold G_ij to within 2^-39 |grad_i| at best, so what falls below that
+ * counts as 0, whatever the other queries' weights are. In drows, grad_i query_i
+ * is held to within 2^-38 of the largest |grad| times the largest |value| of a
+ * query. Results do not depend on timing: no atomics. A non-finite value makes
+ * non-finite what the formulas make so.
  *
  * Both calls only enqueue work on stream, on the current device, can be
  * captured into a graph, and use workspace (device, 256-byte aligned, at
@@ -617,7 +623,7 @@ int			AnnB200SearchTyped(AnnB200TypedJob *jobs, uint32_t n);
  * that work is done; calls that run at the same time need one each. nq <=
  * 2^22, nrows < 2^31, dims <= 65,536. nq 0 does nothing; nrows 0 is
  * ANN_INVALID. If a pipeline wait runs out inside a kernel (4 s), the
- * outputs are NaN.
+ * outputs are NaN (a query without a target keeps its zeros).
  */
 #define ANNB200_BF16 5			/* operands of the calls below; not a shard's
 								 * row format */
@@ -662,7 +668,8 @@ int			AnnB200SoftmaxLossWorkspace(const AnnB200LossJob *job, uint64_t *loss_byte
  *           the index builder's row quantizer, build_cuvs_index.py:296-348,
  *           divides by the scale and sends ties down)
  * A NaN makes its block's scale and codes NaN; an infinity makes the scale
- * infinite and its own code NaN. Enqueued on stream, current device.
+ * infinite and its own code NaN. m < 2^31, k <= 2^20, at most 2^37 - 64 blocks
+ * of 1 x 128 in m x k; m or k 0 does nothing. Enqueued on stream, current device.
  */
 int			AnnB200QuantizeBlocks(uint32_t dtype, const void *x, uint64_t stride, uint64_t m, uint32_t k,
 								  uint32_t square, uint8_t *codes, uint64_t code_stride, float *scales,
@@ -678,7 +685,8 @@ int			AnnB200QuantizeBlocks(uint32_t dtype, const void *x, uint64_t stride, uint
  * a: m rows, b: n rows, of k codes, a_stride / b_stride bytes apart; codes
  * 16-byte aligned, strides multiples of 16. Scales as AnnB200QuantizeBlocks
  * writes them, 1 x 128 or (square != 0) 128 x 128, for each side alone. The
- * sums within a block and over blocks are FP32; out (ANNB200_F32, F16 or
+ * sums within a block and over blocks are FP32, and so is a_scale * b_scale,
+ * which has to be in FP32's normal range for a block to count fully; out (ANNB200_F32, F16 or
  * BF16; rows out_stride values apart) is rounded once. Bytes past k are not
  * read into the sums. m, n < 2^31, k <= 2^20; m or n 0 does nothing, k 0
  * writes zeros. Enqueued on stream, current device; no workspace. A pipeline

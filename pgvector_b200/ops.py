@@ -171,7 +171,8 @@ def _autograd():
 def softmax_loss_grad(queries, rows, targets, lse, grad=None, scale=1.0, need_queries=True, need_rows=True,
                       stream=None):
     """Gradients of sum_i grad_i * loss_i by the queries and the rows, from the
-    inputs of softmax_loss and the lse it returned. grad: float32 [nq], by
+    inputs of softmax_loss and the lse it returned for them (no other: one joined
+    over several calls' rows gives wrong dqueries). grad: float32 [nq], by
     default ones. Returns (dqueries, drows) of the operands' type; None for one
     that is not needed. They are not differentiable further. softmax_loss calls
     this in its backward pass; by hand, ``queries.backward(dqueries)``."""
