@@ -512,9 +512,10 @@ __device__ __forceinline__ void shared_float4(uint32_t addr, float (&v)[4]) {
 // lane would fill the shared-memory port, so the lanes read tensor memory in 8 x
 // 4 patches, where a thread has 4 rows and 32 columns: 9 reads of shared memory
 // a block. Bound by the epilogue: a block's products and loads alone take 720
-// clocks, with the scaling 1,200 (8,191 x 5,000 x 4,096, square: 205 us, 1.63
-// PFLOP/s) and 1,650 (1,024 x 1,000,000 x 1,024: 1,635 us, 1.28 PFLOP/s, where
-// 2 GB of results go out under it). 16 epilogue warps were no faster.
+// clocks, with the scaling 1,260 (8,191 x 5,000 x 4,096, square: 212 us, 1.58
+// PFLOP/s; 219 us a call among calls) and 1,800 (1,024 x 1,000,000 x 1,024: 1,735
+// us, 1.21 PFLOP/s, where 2 GB of results go out under it; 1,905 us among calls,
+// at the lower clocks of steady load). 16 epilogue warps were no faster.
 template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;

@@ -18,11 +18,12 @@
 // rows and queries; in the forward call one a query.
 //
 // What bounds it: the four products, 8 nq n d operations with the logits' second
-// time. 4,096 x 65,536 x 768 bf16, 412 GFLOP each: logits 311 us (the epilogue's
-// 128 exponentials a thread come to 2,048 clocks of the 6,144 a tile's products
-// take, and its other work to about as many again), G 384 us (that, and 128
-// roundings, 64 KB out), dX 271 us, dW 288 us. Below about 256 dimensions the
-// epilogues bound it.
+// time. 4,096 x 65,536 x 768 bf16, 412 GFLOP each: logits 312 us, G 378 us, dX
+// 280 us, dW 292 us. dX and dW run at the product loop's rate. A tile of the
+// logits takes 9,100 clocks and one of G 11,400, where its products and loads
+// alone would take 8,300: the epilogue (128 exponentials a thread, for G 128
+// roundings and 64 KB out too) does not run wholly under the next tile's
+// products. Below about 256 dimensions it bounds the call.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -35,7 +36,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033e-8f;   // log2(e), and what FP32 leaves of it
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial maxima and sums, at most about
+constexpr uint64_t kPartBytes = 256ull << 20;   // the forward call's partial maxima and sums, or those of 256 queries
 constexpr uint64_t kPieceBytes = 512ull << 20;  // G of a piece (128 MB: 4,096 x 65,536 x 768 took 1,538 us for 1,450)
 constexpr uint64_t kMostPieceBytes = 4ull << 30;
 constexpr uint32_t kPlanClusters = 74;          // clusters the plan splits for (148 SMs)
@@ -76,7 +77,7 @@ struct Maxima {
   uint32_t rows[kRowParts], queries[kQueryParts], grad[kGradParts];
   uint32_t all_rows, all_queries;   // joined by the layout kernel
 };
-// The largest of n <= 1024 parts, for every thread of a 256-thread block.
+// The largest of a 256-thread block's values, for each of its threads.
 __device__ __forceinline__ uint32_t block_max(uint32_t best) {
   __shared__ uint32_t top[8];
   best = __reduce_max_sync(0xffffffffu, best);
@@ -87,6 +88,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t best) {
   for (int i = 0; i < 8; i++) best = max(best, top[i]);
   return best;
 }
+// The largest of a grid's parts, for each thread of a 256-thread block.
 __device__ __forceinline__ uint32_t join_parts(const uint32_t *parts, int n) {
   uint32_t best = 0;
   for (int i = threadIdx.x; i < n; i += 256) best = max(best, parts[i]);
