@@ -514,8 +514,8 @@ __device__ __forceinline__ void shared_float4(uint32_t addr, float (&v)[4]) {
 // a block. Bound by the epilogue: a block's products and loads alone take 720
 // clocks, with the scaling 1,260 (8,191 x 5,000 x 4,096, square: 212 us, 1.58
 // PFLOP/s; 219 us a call among calls) and 1,800 (1,024 x 1,000,000 x 1,024: 1,735
-// us, 1.21 PFLOP/s, where 2 GB of results go out under it; 1,905 us among calls,
-// at the lower clocks of steady load). 16 epilogue warps were no faster.
+// us, 1.21 PFLOP/s, where 2 GB of results go out under it; 1,895 us among calls,
+// under the power cap). 16 epilogue warps were no faster.
 template <bool UNIFORM, typename T>
 struct WideOp {
   static constexpr PairKind KIND = PAIR_E4M3;

@@ -19,7 +19,7 @@
 //
 // What bounds it: the four products, 8 nq n d operations with the logits' second
 // time. 4,096 x 65,536 x 768 bf16, 412 GFLOP each: logits 312 us, G 378 us, dX
-// 280 us, dW 292 us. dX and dW run at the product loop's rate. A tile of the
+// 280 us, dW 292 us. dX and dW run near the product loop's rate. A tile of the
 // logits takes 9,100 clocks and one of G 11,400, where its products and loads
 // alone would take 8,300: the epilogue (128 exponentials a thread, for G 128
 // roundings and 64 KB out too) does not run wholly under the next tile's
