@@ -392,7 +392,8 @@ struct BlocksArgs {
   uint32_t mt, nt;          // tiles of a's rows, of b's
   Operands o;
   T *out;
-  int boxes;                // out's rows are 16-byte aligned: `map` stores them
+  int boxes;                // out's rows start on 16-byte boundaries: `map` stores boxes
+  int ragged;               // and do not end on one: not the last box, which would write past n
   CUtensorMap map;
 };
 // Scales a and b both 16-byte aligned, and their rows: loads of four blocks.
@@ -664,7 +665,7 @@ struct WideOp {
             }
           }
         }
-        if (p.boxes) {   // (in 16-bit values)
+        if (p.boxes && !(p.ragged && n0 + (x + 1) * BOX > o.n)) {   // (in 16-bit values)
           box.store(&p.map, (int32_t)((n0 + x * BOX) * (sizeof(T) / 2)), (int32_t)m0);
         } else {
           box.copy(p.out + (uint64_t)m0 * o.out_stride + n0 + x * BOX, o.out_stride,
@@ -686,6 +687,7 @@ cudaError_t launch_tiles(const Operands &o, T *out, bool wide, uint32_t bn, int 
   args.nt = (uint32_t)((o.n + 255) / 256);
   args.boxes = wide && o.out_stride * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
                o.n * sizeof(T) / 2 <= 0x7fffffffull;
+  args.ragged = o.n * sizeof(T) % 16 != 0;
   const bool maps =
       encode_operand_map(args.a, 1, wide ? o.a : o.b, o.k, wide ? o.m : o.n, wide ? o.a_stride : o.b_stride, 128) &&
       encode_operand_map(args.b, 1, wide ? o.b : o.a, o.k, wide ? o.n : o.m, wide ? o.b_stride : o.a_stride, bn / 2) &&

@@ -169,8 +169,9 @@ __device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volati
 
 // A warp's way out to memory: 32 rows of 128 bytes, a row a lane, put into
 // shared memory in the 128-byte swizzle (each 16-byte chunk once: no bank
-// conflicts) and stored as one box by the TMA, whole lines at a time. Rows and
-// columns past the tensor's ends are left out by the TMA.
+// conflicts) and stored as one box by the TMA, whole lines at a time. Rows past
+// the tensor's end are left out by the TMA, columns 16 bytes at a time: a row whose
+// end is not on a 16-byte boundary needs room up to it, or `copy` for its last box.
 constexpr int kBoxBytes = 32 * 128;
 struct BoxStore {
   uint8_t *box;
