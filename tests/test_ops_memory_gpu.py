@@ -124,3 +124,29 @@ def test_blocks_keep_to_their_memory(cuda, m, n, k, out, square):
         got = room.view(dt, (m, stride))
         assert room.guards_are_whole() and torch.equal(got[:, :n], want)
         assert bool((got[:, n:].contiguous().view(torch.uint8) == 0xff).all())
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'float16', 'bfloat16'])
+@pytest.mark.parametrize('nq', [40, 200])
+@pytest.mark.parametrize('dims', [1, 3, 77, 130])
+def test_what_lies_between_the_rows_does_not_count(cuda, dtype, nq, dims):
+    # rows on 16-byte boundaries that end off them, NaN up to the next one
+    import torch
+    import pgvector_b200 as pb
+    dt = getattr(torch, dtype)
+    g = torch.Generator(device='cuda')
+    g.manual_seed(dims)
+    x = torch.randn((nq, dims), generator=g, device='cuda').to(dt)
+    w = torch.randn((900, dims), generator=g, device='cuda').to(dt)
+    t = torch.randint(0, 900, (nq,), generator=g, device='cuda')
+    pad = (dims + 7) // 8 * 8 + 8
+    hx = torch.full((nq, pad), float('nan'), dtype=dt, device='cuda')
+    hw = torch.full((900, pad), float('nan'), dtype=dt, device='cuda')
+    hx[:, :dims], hw[:, :dims] = x, w
+    loss, lse = pb.softmax_loss(x, w, t, scale=0.3)
+    want = (loss, lse) + pb.softmax_loss_grad(x, w, t, lse, scale=0.3)
+    for a, b in ((hx[:, :dims], hw[:, :dims]), (x, hw[:, :dims]), (hx[:, :dims], w)):
+        loss, lse = pb.softmax_loss(a, b, t, scale=0.3)
+        got = (loss, lse) + pb.softmax_loss_grad(a, b, t, lse, scale=0.3)
+        for u, v in zip(got, want):
+            assert torch.equal(u, v)
